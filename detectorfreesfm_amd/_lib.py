@@ -120,6 +120,15 @@ SIGNATURES = [
     ("dfsfm_s2d_front_f32", c_int,
      [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_int,
       c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    ("dfsfm_layernorm_forward", c_int,
+     [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_float, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p]),
+    ("dfsfm_layernorm_backward_workspace", c_size_t, [c_int64, c_int, c_int]),
+    ("dfsfm_layernorm_backward", c_int,
+     [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int,
+      c_void_p, c_size_t, c_void_p]),
+    ("dfsfm_rotary", c_int,
+     [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int, c_int,
+      c_int, c_int, c_float, c_int, c_int64, c_int, c_int, c_int, c_void_p]),
 ]
 
 _lib = None

@@ -1644,3 +1644,181 @@ def maxpool3x3s2_nhwc(x):
     rc = _lib.lib().dfsfm_maxpool3x3s2_nhwc_f32(_ptr(x), None, None, N, H, W, C, _ptr(out), None, None, _stream())
     _lib.check(rc, "dfsfm_maxpool3x3s2_nhwc_f32")
     return out
+
+
+# ---------------------------------------------------------------- layers that are trained (csrc/norm_train.hip, csrc/rotary.hip)
+# fp32, bf16 and fp16 tensors.  Scratch memory comes from torch's allocator call by call, not from ``_workspace``: a captured graph then
+# owns its own, and calls on several streams share none.  The operators record no autograd graph; each has its gradient beside it.
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _dtype_code(what, *ts):
+    if ts[0].dtype not in _DTYPES or any(t is not None and t.dtype != ts[0].dtype for t in ts):
+        raise _lib.DfsfmError(f"{what}: need fp32, bf16 or fp16 tensors of one type")
+    return _DTYPES[ts[0].dtype]
+
+
+def _no_graph(what, *ts):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise _lib.DfsfmError(f"{what}: records no autograd graph: call it on detached tensors (or under torch.no_grad()) and its "
+                              "gradient with the backward function beside it")
+
+
+def _norm_rows(t, what):
+    """(rows, row stride) of [..., C] rows with unit inner stride; copies what does not flatten to uniformly strided rows."""
+    if t.dim() < 1:
+        raise _lib.DfsfmError(f"{what}: need [..., C] tensors")
+    rows = 1
+    for s in t.shape[:-1]:
+        rows *= s
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        t = t.contiguous()
+    dims = [(s, st) for s, st in zip(t.shape[:-1], t.stride()[:-1]) if s != 1]
+    if any(dims[i][1] != dims[i + 1][0] * dims[i + 1][1] for i in range(len(dims) - 1)):
+        t = t.contiguous()
+        return t, rows, t.shape[-1]
+    return t, rows, dims[-1][1] if dims else t.shape[-1]
+
+
+def _norm_affine(what, t, C, *ws):
+    """`wtype` of gamma / beta: the rows' type or fp32, [C], dense."""
+    for w in ws:
+        if w.shape != (C,) or w.dtype != ws[0].dtype or w.dtype not in (t.dtype, torch.float32):
+            raise _lib.DfsfmError(f"{what}: gamma and beta are [C] of one type, the rows' or fp32")
+    return [w.contiguous() for w in ws], _DTYPES[ws[0].dtype]
+
+
+@_on_device
+def layernorm_forward(x, gamma, beta, eps=1e-5, residual=None):
+    """(x - mean) / sqrt(var + eps) * gamma + beta (+ residual) over the last dim of x [..., C], fp32 / bf16 / fp16, C up to 16384; gamma
+    and beta [C] in x's type or fp32.  Returns (y dense in x's type, mean [...], rstd [...] in fp32): what ``layernorm_backward`` reads."""
+    _require_cuda(x, gamma, beta, residual)
+    _no_graph("layernorm_forward", x, gamma, beta, residual)
+    code = _dtype_code("layernorm_forward", x, residual)
+    x, rows, ldx = _norm_rows(x, "layernorm_forward")
+    C = x.shape[-1]
+    (gamma, beta), wtype = _norm_affine("layernorm_forward", x, C, gamma, beta)
+    ldr = 0
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise _lib.DfsfmError("layernorm_forward: the residual has x's shape")
+        residual, _, ldr = _norm_rows(residual, "layernorm_forward")
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean, rstd = torch.empty((2, *x.shape[:-1]), dtype=torch.float32, device=x.device).unbind(0)
+    rc = _lib.lib().dfsfm_layernorm_forward(x.data_ptr(), ldx, gamma.data_ptr(), beta.data_ptr(), wtype, float(eps),
+                                            None if residual is None else residual.data_ptr(), ldr, y.data_ptr(), mean.data_ptr(),
+                                            rstd.data_ptr(), rows, C, code, _stream())
+    _lib.check(rc, "dfsfm_layernorm_forward")
+    return y, mean, rstd
+
+
+@_on_device
+def layernorm_backward(dy, x, mean, rstd, gamma, need_weights=True):
+    """Gradients of ``layernorm_forward`` for dy [..., C]: (dx in x's type, dgamma, dbeta in gamma's type; the two are None without
+    ``need_weights``).  The residual's gradient is dy.  Sums over the rows run in a fixed order: the same call gives the same bits."""
+    _require_cuda(dy, x, mean, rstd, gamma)
+    _no_graph("layernorm_backward", dy, x, gamma)
+    code = _dtype_code("layernorm_backward", x, dy)
+    if dy.shape != x.shape:
+        raise _lib.DfsfmError("layernorm_backward: dy has x's shape")
+    shape = x.shape
+    x, rows, ldx = _norm_rows(x, "layernorm_backward")
+    dy, _, lddy = _norm_rows(dy, "layernorm_backward")
+    C = shape[-1]
+    (gamma,), wtype = _norm_affine("layernorm_backward", x, C, gamma)
+    for t in (mean, rstd):
+        if t.dtype != torch.float32 or t.shape != shape[:-1]:
+            raise _lib.DfsfmError("layernorm_backward: mean and rstd are what layernorm_forward returned for x")
+    mean, rstd = mean.contiguous(), rstd.contiguous()
+    L = _lib.lib()
+    dx = torch.empty(shape, dtype=x.dtype, device=x.device)
+    dg = db = ws = None
+    nbytes = 0
+    if need_weights:
+        dg, db = torch.empty((2, C), dtype=gamma.dtype, device=x.device).unbind(0)
+        nbytes = L.dfsfm_layernorm_backward_workspace(rows, C, code)
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=x.device)
+    rc = L.dfsfm_layernorm_backward(dy.data_ptr(), lddy, x.data_ptr(), ldx, mean.data_ptr(), rstd.data_ptr(), gamma.data_ptr(), wtype,
+                                    dx.data_ptr(), None if dg is None else dg.data_ptr(), None if db is None else db.data_ptr(), rows, C,
+                                    code, None if ws is None else ws.data_ptr(), nbytes, _stream())
+    _lib.check(rc, "dfsfm_layernorm_backward")
+    return dx, dg, db
+
+
+def rotary_frequencies(rotated, base=10000.0, axes=1, scaling="none", factor=1.0, trained=0, device="cuda"):
+    """(inv_freq, amplitude) for ``rotary``: double [rotated / (2 * axes)] angles per position on ``device``, pair p of P turning
+    base^(-p / P) a position, and the factor on the turned values.  ``scaling`` stretches them for sequences ``factor`` times as long
+    as the ``trained`` length: "linear" divides every frequency; "ntk" enlarges the base so that the slowest pair is divided by ``factor``
+    and the fastest stays; "yarn" keeps pairs that turn 32 times or more over the trained length, divides those that turn once or less,
+    blends between, and scales the values by 0.1 ln(factor) + 1."""
+    if axes not in (1, 2) or rotated <= 0 or rotated % (2 * axes) or base <= 0 or factor < 1 or scaling not in ("none", "linear", "ntk", "yarn"):
+        raise _lib.DfsfmError("rotary_frequencies: rotated channels are 2 * axes * pairs, axes 1 or 2, factor >= 1, scaling one of none, "
+                              "linear, ntk, yarn")
+    if scaling == "yarn" and trained <= 0:
+        raise _lib.DfsfmError("rotary_frequencies: yarn needs the trained length")
+    P = rotated // (2 * axes)
+    p = np.arange(P, dtype=np.float64)
+    if scaling == "ntk" and P > 1:
+        base = base * factor ** (P / (P - 1))
+    inv, amplitude = float(base) ** (-p / P), 1.0
+    if scaling == "linear":
+        inv = inv / factor
+    if scaling == "yarn":
+        keep = np.clip(np.log(trained * inv / (2 * np.pi)) / np.log(32.0), 0.0, 1.0)
+        inv, amplitude = inv * keep + inv / factor * (1.0 - keep), 0.1 * float(np.log(factor)) + 1.0
+    return torch.from_numpy(inv).to(device), amplitude
+
+
+def _rotary(what, x, positions, inv_freq, amplitude, axes, interleaved, inplace, backward):
+    _require_cuda(x, positions, inv_freq)
+    _no_graph(what, x)
+    code = _dtype_code(what, x)
+    if x.dim() != 4:
+        raise _lib.DfsfmError(f"{what}: x is [N, L, H, D]")
+    N, L, H, D = x.shape
+    if axes not in (1, 2) or inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not 0 < 2 * axes * inv_freq.numel() <= D:
+        raise _lib.DfsfmError(f"{what}: inv_freq is fp64 [pairs] with 2 * axes * pairs <= D, axes 1 or 2")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise _lib.DfsfmError(f"{what}: positions are int32 or int64")
+    want = (N, L) if axes == 1 else (N, L, axes)
+    if positions.shape != want and positions.shape != want[1:]:
+        raise _lib.DfsfmError(f"{what}: positions are {list(want[1:])} or {list(want)}")
+    positions = positions.to(torch.int64).expand(want)
+    if axes == 1:
+        positions = positions[..., None]
+    inv_freq = inv_freq.contiguous()
+    if inplace:
+        at = 1                              # every element has its own place: strides of the sizes over 1 nest, the smallest first
+        for st, size in sorted((x.stride(i), x.shape[i]) for i in range(4) if x.shape[i] > 1):
+            if st < at:
+                raise _lib.DfsfmError(f"{what}: in-place tensors may not overlap themselves")
+            at = st * size
+        if D > 1 and x.stride(3) != 1:
+            raise _lib.DfsfmError(f"{what}: in-place tensors need a unit channel stride")
+        y = x
+    else:
+        if D > 1 and x.stride(3) != 1:
+            x = x.contiguous()
+        y = torch.empty((N, L, H, D), dtype=x.dtype, device=x.device)
+    rc = _lib.lib().dfsfm_rotary(x.data_ptr(), x.stride(0), x.stride(1), x.stride(2), y.data_ptr(), y.stride(0), y.stride(1), y.stride(2),
+                                 positions.data_ptr(), positions.stride(0), positions.stride(1), positions.stride(2), inv_freq.data_ptr(),
+                                 inv_freq.numel(), axes, 1 if interleaved else 0, 1 if backward else 0, float(amplitude), N, L, H, D, code,
+                                 _stream())
+    _lib.check(rc, "dfsfm_rotary")
+    return y
+
+
+@_on_device
+def rotary(x, positions, inv_freq, amplitude=1.0, axes=1, interleaved=False, inplace=False):
+    """Rotary positions of the heads x [N, L, H, D] (fp32 / bf16 / fp16, strided views OK): each pair of channels turns by position *
+    inv_freq and is scaled by ``amplitude`` (``rotary_frequencies`` makes both).  positions [L] or [N, L], any sign; with ``axes`` = 2
+    (row and column of image tokens) [L, 2] or [N, L, 2], one section of 2 * pairs channels an axis.  Pairs are (p, p + pairs) of a
+    section or, ``interleaved``, (2p, 2p + 1); channels behind the sections stay.  Returns a dense tensor, or x changed ``inplace``.
+    q and k that are columns of one projection turn in one call on their common view."""
+    return _rotary("rotary", x, positions, inv_freq, amplitude, axes, interleaved, inplace, False)
+
+
+@_on_device
+def rotary_backward(dy, positions, inv_freq, amplitude=1.0, axes=1, interleaved=False, inplace=False):
+    """Gradient of ``rotary`` for its result's gradient dy: the same turn the other way."""
+    return _rotary("rotary_backward", dy, positions, inv_freq, amplitude, axes, interleaved, inplace, True)

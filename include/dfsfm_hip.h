@@ -33,6 +33,11 @@ extern "C" {
 #define DFSFM_E_WORKSPACE (-3)   /* workspace too small (query the *_workspace function)   */
 #define DFSFM_E_LAUNCH (-4)      /* hipLaunch / runtime error; see dfsfm_last_error_string */
 
+/* Element types of the entry points that take a `dtype` (and a weights' type `wtype`). */
+#define DFSFM_F32 0
+#define DFSFM_BF16 1
+#define DFSFM_F16 2
+
 /* Library / device introspection. */
 int dfsfm_version(void);                    /* ABI version, currently 1 */
 const char* dfsfm_last_error_string(void);  /* thread-local text for the last DFSFM_E_LAUNCH */
@@ -215,6 +220,30 @@ int dfsfm_dwconv3x3_nhwc_f32(const float* x, int N, int H, int W, int C, const f
 /* F.interpolate(mode='bilinear', align_corners=True) of NHWC fp32 maps (FPN top-down path, match_LA_large.py:232-236).
  * x [N,hin,win,C] -> out [N,hout,wout,C]; C % 4 == 0. */
 int dfsfm_bilinear_up_nhwc_f32(const float* x, int N, int hin, int win, int C, int hout, int wout, float* out, void* stream);
+
+/* ---- Layers that are trained: fp32, bf16 or fp16 tensors (`dtype`), 32-bit sums, no atomics: a call's bits do not change -------- */
+
+/* Layer norm that keeps its rows' statistics: y = (x - mean) * rstd * gamma + beta (+ residual), rstd = 1 / sqrt(var + eps) with the
+ * biased variance.  x, residual [rows, C] with row strides ldx, ldr in elements (0: one row for all); gamma, beta [C] in `wtype`
+ * (the dtype, or DFSFM_F32); y [rows, C] dense; mean, rstd [rows].  Any C up to 16384, any alignment. */
+int dfsfm_layernorm_forward(const void* x, int64_t ldx, const void* gamma, const void* beta, int wtype, float eps, const void* residual,
+                            int64_t ldr, void* y, float* mean, float* rstd, int64_t rows, int C, int dtype, void* stream);
+
+/* Its gradient: dx [rows, C] dense and, unless both are null, dgamma, dbeta [C] in `wtype` (zeros for rows = 0).  The residual's
+ * gradient is dy itself.  The workspace is needed for dgamma and dbeta alone. */
+size_t dfsfm_layernorm_backward_workspace(int64_t rows, int C, int dtype);
+int dfsfm_layernorm_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* mean, const float* rstd,
+                             const void* gamma, int wtype, void* dx, void* dgamma, void* dbeta, int64_t rows, int C, int dtype,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rotary positions: pair (a, b) of a head's channels -> amplitude * (a cos t - b sin t, b cos t + a sin t), t = position * inv_freq;
+ * backward != 0 turns by -t (the gradient).  x, y [N, L, H, D] with element strides (n, l, h) and unit channel stride; y is another
+ * tensor or x itself with x's strides.  positions: int64 [N, L, axes] with element strides (0: broadcast), of any sign; inv_freq:
+ * double [pairs].  The first 2 * pairs * axes channels are `axes` (1 or 2) sections of 2 * pairs, each turned by its axis's position:
+ * pair p of a section is (p, p + pairs), or (2 p, 2 p + 1) if `interleaved`.  The channels behind are copied.  D <= 512. */
+int dfsfm_rotary(const void* x, int64_t xn, int64_t xl, int64_t xh, void* y, int64_t yn, int64_t yl, int64_t yh,
+                 const int64_t* positions, int64_t pn, int64_t pl, int64_t pa, const double* inv_freq, int pairs, int axes, int interleaved,
+                 int backward, float amplitude, int N, int64_t L, int H, int D, int dtype, void* stream);
 
 /* ---- ASpanFormer coarse matcher (third_party/aspantransformer/src/ASpanFormer/) ------------------
  * Maps are NHWC fp32 with a row (= token) pitch in floats, so column slices of wider buffers can be read and written. */
