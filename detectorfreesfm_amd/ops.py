@@ -1822,3 +1822,83 @@ def rotary(x, positions, inv_freq, amplitude=1.0, axes=1, interleaved=False, inp
 def rotary_backward(dy, positions, inv_freq, amplitude=1.0, axes=1, interleaved=False, inplace=False):
     """Gradient of ``rotary`` for its result's gradient dy: the same turn the other way."""
     return _rotary("rotary_backward", dy, positions, inv_freq, amplitude, axes, interleaved, inplace, True)
+
+
+def _attention_args(what, q, k, v, kv_lens, kv_mask, scale):
+    """Checked tensors of a cross attention call: (q, k, v, lens int32, mask uint8, scale, sizes, dtype code)."""
+    _require_cuda(q, k, v, kv_lens, kv_mask)
+    code = _dtype_code(what, q, k, v)
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise _lib.DfsfmError(f"{what}: need q [N, L, H, D] and k, v [N, S, Hkv, D]")
+    (N, L, H, D), (S, Hkv) = q.shape, k.shape[1:3]
+    if D == 0 or D > 128 or D % 8 or (H % Hkv if Hkv else H):
+        raise _lib.DfsfmError(f"{what}: head dims are multiples of 8 up to 128, query heads a multiple of the key heads")
+    if kv_lens is not None:
+        if kv_lens.shape != (N,) or kv_lens.dtype not in (torch.int32, torch.int64):
+            raise _lib.DfsfmError(f"{what}: kv_lens is int32 or int64 [N]")
+        kv_lens = kv_lens.clamp(0, S).to(torch.int32) if kv_lens.dtype == torch.int64 else kv_lens
+        kv_lens = kv_lens.contiguous()
+    if kv_mask is not None:
+        if kv_mask.shape != (N, S):
+            raise _lib.DfsfmError(f"{what}: kv_mask is [N, S]")
+        kv_mask = _as_u8(kv_mask)
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise _lib.DfsfmError(f"{what}: the scale is positive")
+    q, k, v = (t if t.stride(3) == 1 else t.contiguous() for t in (q, k, v))
+    return q, k, v, kv_lens, kv_mask, scale, (N, L, S, H, Hkv, D), code
+
+
+def _heads_ptr(t):
+    s = t.stride()
+    return t.data_ptr(), s[0], s[1], s[2]
+
+
+@_on_device
+def cross_attention(q, k, v, kv_lens=None, kv_mask=None, scale=None):
+    """softmax(scale * q k^T) v of q [N, L, H, D] over states k, v [N, S, Hkv, D] of another length, fp32 / bf16 / fp16, D a multiple of 8
+    up to 128, strided views OK (unit channel stride); query heads h * H / Hkv ... share key head h.  Sequence n looks at its keys s <
+    kv_lens[n] (int tensor on the device, clamped to 0 .. S) with kv_mask[n, s] true; what padded places hold, NaN included, does not
+    matter, and a sequence without keys gives zeros.  ``scale`` defaults to D ** -0.5.  L = 1 is the single-token form: the keys are
+    split over the chip and joined.  Returns (out [N, L, H, D] dense, lse [N, H, L] fp32: the scores' log-sum-exp, -inf without keys)."""
+    _no_graph("cross_attention", q, k, v)
+    q, k, v, kv_lens, kv_mask, scale, sizes, code = _attention_args("cross_attention", q, k, v, kv_lens, kv_mask, scale)
+    N, L, S, H, Hkv, D = sizes
+    out = torch.empty((N, L, H, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((N, H, L), dtype=torch.float32, device=q.device)
+    lib = _lib.lib()
+    nbytes = lib.dfsfm_cross_attention_workspace(*sizes)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=q.device) if nbytes else None
+    rc = lib.dfsfm_cross_attention(*_heads_ptr(q), *_heads_ptr(k), *_heads_ptr(v), None if kv_lens is None else kv_lens.data_ptr(),
+                                   None if kv_mask is None else kv_mask.data_ptr(), out.data_ptr(), lse.data_ptr(), *sizes, scale, code,
+                                   None if ws is None else ws.data_ptr(), nbytes, _stream())
+    _lib.check(rc, "dfsfm_cross_attention")
+    return out, lse
+
+
+@_on_device
+def cross_attention_backward(dout, q, k, v, out, lse, kv_lens=None, kv_mask=None, scale=None):
+    """Gradients (dq, dk, dv), dense, of ``cross_attention`` for dout [N, L, H, D]; out and lse are what it returned, the other arguments
+    what it was called with.  Keys that are not there get zeros.  Sums run in a fixed order: the same call gives the same bits.
+    fp16: products p * ds are carried with a power of two per column, so gradients far below fp16's normal range keep their digits."""
+    _no_graph("cross_attention_backward", dout, q, k, v)
+    q, k, v, kv_lens, kv_mask, scale, sizes, code = _attention_args("cross_attention_backward", q, k, v, kv_lens, kv_mask, scale)
+    _require_cuda(dout, out, lse)
+    N, L, S, H, Hkv, D = sizes
+    if _dtype_code("cross_attention_backward", q, dout, out) != code or dout.shape != q.shape or out.shape != q.shape:
+        raise _lib.DfsfmError("cross_attention_backward: dout and out have q's shape and type")
+    if lse.shape != (N, H, L) or lse.dtype != torch.float32:
+        raise _lib.DfsfmError("cross_attention_backward: lse is what cross_attention returned, fp32 [N, H, L]")
+    dout, out, lse = (t if t.stride(-1) == 1 else t.contiguous() for t in (dout, out, lse))
+    lse = lse.contiguous()
+    dq = torch.empty((N, L, H, D), dtype=q.dtype, device=q.device)
+    dk, dv = (torch.empty((N, S, Hkv, D), dtype=q.dtype, device=q.device) for _ in range(2))
+    lib = _lib.lib()
+    nbytes = lib.dfsfm_cross_attention_backward_workspace(*sizes)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=q.device)
+    rc = lib.dfsfm_cross_attention_backward(*_heads_ptr(dout), *_heads_ptr(q), *_heads_ptr(k), *_heads_ptr(v), *_heads_ptr(out),
+                                            lse.data_ptr(), None if kv_lens is None else kv_lens.data_ptr(),
+                                            None if kv_mask is None else kv_mask.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                            *sizes, scale, code, ws.data_ptr(), nbytes, _stream())
+    _lib.check(rc, "dfsfm_cross_attention_backward")
+    return dq, dk, dv

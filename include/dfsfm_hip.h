@@ -245,6 +245,27 @@ int dfsfm_rotary(const void* x, int64_t xn, int64_t xl, int64_t xh, void* y, int
                  const int64_t* positions, int64_t pn, int64_t pl, int64_t pa, const double* inv_freq, int pairs, int axes, int interleaved,
                  int backward, float amplitude, int N, int64_t L, int H, int D, int dtype, void* stream);
 
+/* Softmax attention of q [N, L, H, D] over an encoder's states k, v [N, S, Hkv, D] of another length (element strides n, length, head;
+ * unit channel stride; any alignment; D a multiple of 8 up to 128; H a multiple of Hkv, query head h reads key head h / (H / Hkv)):
+ * out [N, L, H, D] dense = softmax(scale * q k^T) v and lse [N, H, L] = log sum exp(scale * q k^T) in fp32, over the keys s < kv_lens[n]
+ * (int32, clamped to 0 .. S; null: all) with kv_mask[n, s] != 0 (uint8, dense [N, S]; null: all).  What k and v hold elsewhere is not
+ * looked at, NaN included.  A query without keys gets out = 0, lse = -inf.  scale > 0. */
+size_t dfsfm_cross_attention_workspace(int N, int L, int S, int H, int Hkv, int D);
+int dfsfm_cross_attention(const void* q, int64_t qn, int64_t ql, int64_t qh, const void* k, int64_t kn, int64_t ks, int64_t kh,
+                          const void* v, int64_t vn, int64_t vs, int64_t vh, const int* kv_lens, const uint8_t* kv_mask, void* out,
+                          float* lse, int N, int L, int S, int H, int Hkv, int D, float scale, int dtype, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* Its gradient for dout [N, L, H, D] from the forward pass's out and lse: dq [N, L, H, D], dk, dv [N, S, Hkv, D], dense, in the dtype; the
+ * gradients of shared key heads are sums over their query heads; keys that are not there get zeros.  kv_lens, kv_mask and scale are the
+ * forward pass's. */
+size_t dfsfm_cross_attention_backward_workspace(int N, int L, int S, int H, int Hkv, int D);
+int dfsfm_cross_attention_backward(const void* dout, int64_t gn, int64_t gl, int64_t gh, const void* q, int64_t qn, int64_t ql, int64_t qh,
+                                   const void* k, int64_t kn, int64_t ks, int64_t kh, const void* v, int64_t vn, int64_t vs, int64_t vh,
+                                   const void* out, int64_t on, int64_t ol, int64_t oh, const float* lse, const int* kv_lens,
+                                   const uint8_t* kv_mask, void* dq, void* dk, void* dv, int N, int L, int S, int H, int Hkv, int D,
+                                   float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- ASpanFormer coarse matcher (third_party/aspantransformer/src/ASpanFormer/) ------------------
  * Maps are NHWC fp32 with a row (= token) pitch in floats, so column slices of wider buffers can be read and written. */
 

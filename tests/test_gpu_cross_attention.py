@@ -1,0 +1,313 @@
+"""Cross attention with its gradient on the GPU (csrc/cross_attention.hip) against its formula in 64 bits.
+
+Bounds (``reference``).  u = 2^-24, ut half a step of the tensors' type.  A score is a 32-bit sum of D products: off by es = (D + 2) u scale
+<|q|, |k|>.  Its exponential's argument is rounded twice at its own size and the maximum's (or lse's), the exponential by two ulp: a weight is
+off by ep = 2 es + 6 u (|s| + |lse| + 1) of itself, and is rounded to the type once more before its product (ut; fp16 weights below 2^-14 by
+2^-25 of the row's largest).  Sums over n rows add (n + 8) u of their absolute terms: a chain is the worst order.  The gradient's factors
+follow the same way, delta with the type's rounding of `out` in it; fp16 products p * ds are carried with a power of two that puts the
+column's largest at 2^11 or above, so their floor of 2^-25 is 2^-36 of it.
+"""
+import math
+
+import pytest
+import torch
+
+from detectorfreesfm_amd import _lib, ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def rounded(ref, bound, t):
+    """+ half a step of the type: eps / 2 of the value, half the subnormals' spacing below the smallest normal number."""
+    f = torch.finfo(t)
+    return bound + torch.clamp(f.eps / 2 * (ref.abs() + bound), min=f.eps * f.smallest_normal / 2)
+
+
+def close(got, ref, bound, what):
+    assert got.shape == ref.shape, what
+    got = got.double().cpu()
+    same = (got == ref) | (torch.isnan(got) & torch.isnan(ref))
+    bad = ~same & ~((got - ref).abs() <= bound)
+    assert not bool(bad.any()), (what, int(bad.sum()), (got - ref).abs()[bad].max().item(), bound[bad].min().item())
+
+
+def make(N, L, S, H, Hkv, D, t, mask, seed, q_scale=1.5, g_scale=1.0):
+    """Inputs on the CPU; padded places hold NaN, inf and the type's lowest value."""
+    g = torch.Generator().manual_seed(seed)
+    q, k, v, do = ((torch.randn(s, generator=g) * f).to(t) for s, f in (((N, L, H, D), q_scale), ((N, S, Hkv, D), 1.0), ((N, S, Hkv, D), 1.0),
+                                                                       ((N, L, H, D), g_scale)))
+    lens = km = None
+    there = torch.ones((N, S), dtype=torch.bool)
+    if mask in ("lens", "both"):
+        lens = torch.tensor([[S, (S + 1) // 2, 0, S // 3, -4, S + 9][(i + seed) % 6] for i in range(N)], dtype=torch.int32)
+        there &= torch.arange(S)[None] < lens[:, None]
+    if mask in ("mask", "both"):
+        km = torch.rand((N, S), generator=g) < 0.7
+        if S > 130:
+            km[:, 64:128] = False                     # a whole tile
+        there &= km
+    junk = torch.tensor([float("nan"), float("inf"), torch.finfo(t).min]).to(t)[torch.arange(S) % 3][None, :, None, None]
+    k, v = (torch.where(there[..., None, None], x, junk) for x in (k, v))
+    return q, k, v, do, lens, km, there
+
+
+def reference(q, k, v, do, there, scale, out_type, got_out=None):
+    """{name: (64-bit value, bound before the last rounding)}"""
+    t = q.dtype
+    ut = 0.0 if t == torch.float32 else torch.finfo(t).eps / 2
+    fp16 = t == torch.float16
+    G = q.shape[2] // k.shape[2]
+    N, L, H, D = q.shape
+    S = k.shape[1]
+    z = there[:, :, None, None]
+    Q, DO = (x.double().permute(0, 2, 1, 3) for x in (q, do))
+    K, V = (torch.where(z, x.double(), 0.0).permute(0, 2, 1, 3).repeat_interleave(G, 1) for x in (k, v))
+    s = scale * Q @ K.transpose(2, 3)
+    dead = ~there[:, None, None, :]
+    lse = torch.logsumexp(s.masked_fill(dead, -math.inf), -1) if S else torch.full((N, H, L), -math.inf, dtype=torch.float64)
+    lse0 = torch.where(lse == -math.inf, 0.0, lse)[..., None]
+    p = torch.exp(s - lse0).masked_fill(dead, 0.0)
+    out = p @ V
+    es = (D + 2) * U * scale * (Q.abs() @ K.abs().transpose(2, 3))
+    es = es.masked_fill(dead, 0.0)
+    # one maximum of all keys' errors a row: the normalisation mixes them
+    ep = (2 * es + 6 * U * (s.abs().masked_fill(dead, 0.0) + lse0.abs() + 1)).amax(-1, keepdim=True) if S else torch.zeros(N, H, L, 1).double()
+    top = torch.exp(s.masked_fill(dead, -math.inf).amax(-1, keepdim=True) - lse0) if S else ep
+    ob = (p @ V.abs()) * (2 * ep + ut + (S + 8) * U)
+    if fp16 and S:
+        ob = ob + 2.0 ** -25 * top * V.abs().sum(-2, keepdim=True)
+    r = {"out": (out, ob), "lse": (lse, ep[..., 0] + (S + 8) * U)}
+    dp = DO @ V.transpose(2, 3)
+    delta = (DO * out).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    e_dp = (D + 2) * U * (DO.abs() @ V.abs().transpose(2, 3))
+    e_delta = (DO.abs() * (ob + torch.finfo(t).eps / 2 * (out.abs() + ob) + (D + 2) * U * out.abs())).sum(-1, keepdim=True)
+    if fp16:
+        e_delta = e_delta + 2.0 ** -25 * DO.abs().sum(-1, keepdim=True)
+    eds = p * (e_dp + e_delta + 2 * U * (dp.abs() + delta.abs())) + ds.abs() * 3 * ep
+    wide = eds + (ut + 2 * U) * (ds.abs() + eds)
+    R = L * G
+    qb = wide @ K.abs() + (S + 8) * U * (ds.abs() @ K.abs())
+    kb = wide.transpose(2, 3) @ Q.abs() + (R + 8) * U * (ds.abs().transpose(2, 3) @ Q.abs())
+    vb = ((p * (3 * ep + ut + 2 * U)).transpose(2, 3) + (R + 8) * U * p.transpose(2, 3)) @ DO.abs()
+    if fp16 and S:
+        big = (ds.abs() + eds)
+        qb = qb + 2.0 ** -36 * big.amax(-1, keepdim=True) * K.abs().sum(-2, keepdim=True)
+        # a key's floor goes by the largest of all the rows that share its head
+        kmax = big.amax(-2, keepdim=True).reshape(N, H // G, G, 1, S).amax(2).repeat_interleave(G, 1).transpose(2, 3)
+        kb = kb + 2.0 ** -36 * kmax * Q.abs().sum(-2, keepdim=True)
+        vb = vb + 2.0 ** -39 * DO.abs().sum(-2, keepdim=True)
+    def shared(x):
+        return x.reshape(N, H // G, G, S, D).sum(2).permute(0, 2, 1, 3)
+    gone = there[:, :, None, None]
+    r["out"] = tuple(x.permute(0, 2, 1, 3) for x in r["out"])
+    r["dq"] = tuple(scale * x.permute(0, 2, 1, 3) for x in (ds @ K, qb))
+    r["dk"] = tuple(torch.where(gone, scale * shared(x), 0.0) for x in (ds.transpose(2, 3) @ Q, kb))
+    r["dv"] = tuple(torch.where(gone, shared(x), 0.0) for x in (p.transpose(2, 3) @ DO, vb))
+    return r
+
+
+def both(q, k, v, do, lens, km, scale=None):
+    dev = [None if x is None else x.to(DEV) for x in (q, k, v, do, lens, km)]
+    out, lse = ops.cross_attention(*dev[:3], kv_lens=dev[4], kv_mask=dev[5], scale=scale)
+    dq, dk, dv = ops.cross_attention_backward(dev[3], *dev[:3], out, lse, kv_lens=dev[4], kv_mask=dev[5], scale=scale)
+    return {"out": out, "lse": lse, "dq": dq, "dk": dk, "dv": dv}
+
+
+def check(got, q, k, v, do, there, scale, what):
+    ref = reference(q, k, v, do, there, scale, q.dtype)
+    for name, (value, bound) in ref.items():
+        close(got[name], value, bound if name == "lse" else rounded(value, bound, q.dtype), (name, what))
+        assert got[name].dtype == (torch.float32 if name == "lse" else q.dtype)
+
+
+SHAPES = [(1, 1, 1, 1, 1, 8), (6, 7, 5, 4, 2, 32), (1, 33, 64, 2, 1, 16), (2, 130, 65, 3, 3, 40), (2, 129, 200, 8, 2, 64), (6, 64, 63, 4, 4, 80),
+          (1, 100, 257, 2, 2, 128), (3, 1, 700, 8, 1, 64), (1, 300, 1, 2, 1, 32), (2, 2, 3001, 2, 2, 128), (2, 2000, 20, 2, 1, 24),
+          (1, 257, 513, 5, 1, 96), (2, 31, 129, 7, 7, 120)]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("mask", ["none", "lens", "mask", "both"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_cross_attention_shapes(built_lib, shape, mask, t):
+    q, k, v, do, lens, km, there = make(*shape, t, mask, seed=sum(shape) + len(mask))
+    check(both(q, k, v, do, lens, km), q, k, v, do, there, shape[-1] ** -0.5, (shape, mask, t))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("scale", [0.02, 1.0])
+def test_cross_attention_scales(built_lib, t, scale):
+    """Flat and nearly one-hot rows."""
+    q, k, v, do, lens, km, there = make(2, 90, 333, 4, 2, 64, t, "lens", 3, q_scale=2.0)
+    check(both(q, k, v, do, lens, km, scale), q, k, v, do, there, scale, (t, scale))
+
+
+@pytest.mark.parametrize("g_scale", [1e-2, 1.0, 200.0])
+def test_cross_attention_fp16_gradients_of_any_size(built_lib, g_scale):
+    """p * ds down to 1e-8 of fp16's range and up to its end: the gradients keep fp16's digits."""
+    q, k, v, do, lens, km, there = make(1, 500, 1500, 2, 1, 32, torch.float16, "none", 4, g_scale=g_scale)
+    do[:, ::7] *= 0.01
+    do[:, 100:200] *= 8.0
+    check(both(q, k, v, do, lens, km), q, k, v, do, there, 32 ** -0.5, g_scale)
+
+
+def test_cross_attention_differences(built_lib):
+    """dq, dk, dv against central differences of the 64-bit forward pass."""
+    q, k, v, do, lens, km, there = make(1, 5, 9, 4, 2, 16, torch.float32, "mask", 5)
+    got = both(q, k, v, do, lens, km)
+    g = torch.Generator().manual_seed(6)
+    xs = [torch.where(there[..., None, None], x, torch.zeros(())).double() if i else x.double() for i, x in enumerate((q, k, v))]
+
+    def loss(q, k, v):
+        a = torch.einsum("nlhd,nshd->nhls", q, k.repeat_interleave(2, 2)) / 4.0
+        p = torch.softmax(a.masked_fill(~there[:, None, None], -math.inf), -1)
+        return (torch.einsum("nhls,nshd->nlhd", p, v.repeat_interleave(2, 2)) * do.double()).sum()
+
+    for i, name in enumerate(("dq", "dk", "dv")):
+        for _ in range(15):
+            at = tuple(int(torch.randint(0, s, (1,), generator=g)) for s in xs[i].shape)
+            hi, lo = [x.clone() for x in xs], [x.clone() for x in xs]
+            hi[i][at] += 1e-6
+            lo[i][at] -= 1e-6
+            d = (loss(*hi) - loss(*lo)) / 2e-6
+            assert abs(float(got[name][at]) - float(d)) < 1e-5, (name, at)      # 32-bit sums of ~16 terms of size 1; differences 1e-9
+
+
+def test_cross_attention_views(built_lib):
+    """Columns of fused projections, head-major tensors, a shared encoder batch (stride 0), odd offsets: as the dense tensors."""
+    g = torch.Generator().manual_seed(7)
+    N, L, S, H, D = 3, 70, 90, 4, 32
+    for t in TYPES:
+        fused = torch.randn((N, S, 3 * H * D + 1), generator=g).to(t).to(DEV)
+        k, v = (fused[..., o:o + H * D].unflatten(-1, (H, D)) for o in (1, H * D + 1))
+        q = torch.randn((N, H, L, D), generator=g).to(t).to(DEV).transpose(1, 2)
+        do = torch.randn((N, L, H, D + 3), generator=g).to(t).to(DEV)[..., 3:]
+        mask = torch.rand((N, S + 5), generator=g).to(DEV)[:, 5:] < 0.8
+        enc = torch.randn((1, S, H, D), generator=g).to(t).to(DEV).expand(N, S, H, D)
+        for kk, vv in ((k, v), (enc, v), (v.transpose(0, 1).contiguous().transpose(0, 1), enc)):
+            a = [q, kk, vv]
+            b = [x.clone(memory_format=torch.contiguous_format) for x in a]
+            (o1, l1), (o2, l2) = (ops.cross_attention(*x, kv_mask=mask) for x in (a, b))
+            assert torch.equal(o1, o2) and torch.equal(l1, l2)
+            g1 = ops.cross_attention_backward(do, *a, o1, l1, kv_mask=mask)
+            g2 = ops.cross_attention_backward(do.contiguous(), *b, o2.transpose(1, 2).contiguous().transpose(1, 2), l2, kv_mask=mask.clone())
+            assert all(torch.equal(x, y) for x, y in zip(g1, g2))
+        strided = torch.randn((N, L, H, 2 * D), generator=g).to(t).to(DEV)[..., ::2]
+        assert torch.equal(ops.cross_attention(strided, k, v)[0], ops.cross_attention(strided.contiguous(), k, v)[0])
+
+
+def test_cross_attention_long_offsets(built_lib):
+    """Key offsets behind 2^31 elements, in the single-token form and in the gradient."""
+    S, row = 600, 4_000_000
+    big = torch.zeros((S * row,), dtype=torch.bfloat16, device=DEV)
+    g = torch.Generator().manual_seed(8)
+    k, v = (torch.as_strided(big, (1, S, 2, 64), (0, row, 64, 1), storage_offset=o) for o in (0, 128))
+    kd, vd = (torch.randn((1, S, 2, 64), generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    k.copy_(kd)
+    v.copy_(vd)
+    q, do = (torch.randn((1, 3, 4, 64), generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    out, lse = ops.cross_attention(q, k, v)
+    ref = ops.cross_attention(q, kd, vd)
+    assert torch.equal(out, ref[0]) and torch.equal(lse, ref[1])
+    assert all(torch.equal(a, b) for a, b in zip(ops.cross_attention_backward(do, q, k, v, out, lse),
+                                                 ops.cross_attention_backward(do, q, kd, vd, out, lse)))
+
+
+def test_cross_attention_empty(built_lib):
+    for N, L, S in ((0, 3, 4), (2, 0, 4), (2, 3, 0)):
+        q, k = torch.randn((N, L, 4, 32), device=DEV), torch.randn((N, S, 2, 32), device=DEV)
+        out, lse = ops.cross_attention(q, k, k)
+        assert out.shape == q.shape and float(out.abs().sum()) == 0 and bool((lse == -math.inf).all())
+        dq, dk, dv = ops.cross_attention_backward(q, q, k, k, out, lse)
+        assert dq.shape == q.shape and dk.shape == k.shape and all(float(x.abs().sum()) == 0 for x in (dq, dk, dv))
+    q, k = torch.randn((2, 3, 4, 32), device=DEV), torch.full((2, 5, 2, 32), float("nan"), device=DEV)
+    for kw in ({"kv_lens": torch.zeros(2, dtype=torch.int64, device=DEV)}, {"kv_mask": torch.zeros((2, 5), dtype=torch.bool, device=DEV)}):
+        out, lse = ops.cross_attention(q, k, k, **kw)
+        assert float(out.abs().sum()) == 0 and bool((lse == -math.inf).all())
+        assert all(float(x.abs().sum()) == 0 for x in ops.cross_attention_backward(q, q, k, k, out, lse, **kw))
+
+
+def test_cross_attention_nan_stays_in_its_row(built_lib):
+    q, k = torch.randn((1, 50, 2, 32), device=DEV), torch.randn((1, 80, 2, 32), device=DEV)
+    ref = ops.cross_attention(q, k, k)
+    bad = q.clone()
+    bad[0, 7, 1] = float("nan")
+    out, lse = ops.cross_attention(bad, k, k)
+    assert bool(out[0, 7, 1].isnan().all()) and bool(lse[0, 1, 7].isnan())
+    out[0, 7, 1], lse[0, 1, 7] = ref[0][0, 7, 1], ref[1][0, 1, 7]
+    assert torch.equal(out, ref[0]) and torch.equal(lse, ref[1])
+
+
+def test_cross_attention_values_at_the_range_s_end(built_lib):
+    """A mean of values at fp16's largest is that value, not infinity (weights are rounded, their sum is not); an infinite one stays."""
+    for L, S in ((1, 2000), (70, 300)):
+        q, k = (torch.randn(s, device=DEV).half() for s in ((1, L, 2, 64), (1, S, 2, 64)))
+        v = torch.full_like(k, 65504.0)
+        v[:, :, 1] = -65504.0
+        v[0, 0, 0, 0] = float("inf")
+        out, _ = ops.cross_attention(q, k, v)
+        assert bool((out[:, :, 0, 1:] == 65504).all()) and bool((out[:, :, 1] == -65504).all()) and bool((out[:, :, 0, 0] == math.inf).all())
+
+
+@pytest.mark.parametrize("shape", [(2, 1, 2000, 4, 4, 64), (1, 1500, 40, 2, 1, 64), (2, 200, 300, 4, 2, 128)])
+def test_cross_attention_same_bits_and_streams(built_lib, shape):
+    q, k, v, do, lens, km, _ = (None if x is None else x.to(DEV) for x in make(*shape, torch.bfloat16, "both", 9))
+    ref = both(q, k, v, do, lens, km)
+    torch.cuda.synchronize()
+    outs = []
+    for s in [torch.cuda.Stream() for _ in range(3)]:
+        with torch.cuda.stream(s):
+            outs.append(both(q, k, v, do, lens, km))
+    torch.cuda.synchronize()
+    for o in outs:
+        assert all(torch.equal(o[n], ref[n]) for n in ref)
+
+
+@pytest.mark.parametrize("L", [1, 150])
+def test_cross_attention_graphs(built_lib, L):
+    """Two graphs with their own scratch memory, replayed on two streams at once with new lengths and inputs, against eager calls."""
+    cases, graphs, outs = [], [], []
+    for i in range(2):
+        c = [None if x is None else x.to(DEV) for x in make(2, L, 1200, 4, 2, 64, torch.float16, "lens", 10 + i)[:6]]
+        c[1], c[2] = torch.nan_to_num(c[1], nan=1.0, posinf=1.0, neginf=-1.0), torch.nan_to_num(c[2], nan=1.0, posinf=1.0, neginf=-1.0)
+        both(*c)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(both(*c))
+        cases.append(c)
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for k in range(3):
+        for c in cases:
+            c[0].mul_(0.9)
+            c[4].copy_(torch.tensor([400 + 300 * k, 1 + k], dtype=torch.int32))
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for c, o in zip(cases, outs):
+            ref = both(*c)
+            assert all(torch.equal(o[n], ref[n]) for n in ref)
+
+
+def test_cross_attention_refusals(built_lib):
+    q, k = torch.randn((2, 3, 4, 32), device=DEV), torch.randn((2, 5, 2, 32), device=DEV)
+    out, lse = ops.cross_attention(q, k, k)
+    lens, mask = torch.tensor([3, 2], device=DEV), torch.ones((2, 5), dtype=torch.bool, device=DEV)
+    bad = [lambda: ops.cross_attention(q, k, k[:, :4]), lambda: ops.cross_attention(q, k.half(), k.half()), lambda: ops.cross_attention(q, k[:1], k[:1]),
+           lambda: ops.cross_attention(q[:, :, :3], k, k), lambda: ops.cross_attention(q[..., :12], k[..., :12], k[..., :12]),
+           lambda: ops.cross_attention(*(torch.randn((2, 3, 4, 136), device=DEV),) * 3), lambda: ops.cross_attention(q.double(), k.double(), k.double()),
+           lambda: ops.cross_attention(q, k, k, kv_lens=lens[:1]), lambda: ops.cross_attention(q, k, k, kv_lens=lens.float()),
+           lambda: ops.cross_attention(q, k, k, kv_lens=lens.cpu()), lambda: ops.cross_attention(q, k, k, kv_mask=mask[:, :4]),
+           lambda: ops.cross_attention(q, k, k, scale=0.0), lambda: ops.cross_attention(q, k, k, scale=float("nan")),
+           lambda: ops.cross_attention(q[0], k[0], k[0]), lambda: ops.cross_attention(q.clone().requires_grad_(), k, k),
+           lambda: ops.cross_attention_backward(q[:, :2], q, k, k, out, lse), lambda: ops.cross_attention_backward(q.half(), q, k, k, out, lse),
+           lambda: ops.cross_attention_backward(q, q, k, k, out, lse.transpose(1, 2)), lambda: ops.cross_attention_backward(q, q, k, k, out, lse.half())]
+    for call in bad:
+        with pytest.raises(_lib.DfsfmError):
+            call()
