@@ -1646,102 +1646,127 @@ def maxpool3x3s2_nhwc(x):
     return out
 
 
-# ---------------------------------------------------------------- layers that are trained (csrc/norm_train.hip, csrc/rotary.hip)
-# fp32, bf16 and fp16 tensors.  Scratch memory comes from torch's allocator call by call, not from ``_workspace``: a captured graph then
-# owns its own, and calls on several streams share none.  The operators record no autograd graph; each has its gradient beside it.
+# ---------------------------------------------------------------- layers that are trained (csrc/norm_train.hip, rotary.hip,
+# cross_attention.hip): fp32, bf16 and fp16 tensors.  Scratch memory comes from torch's allocator call by call, not from ``_workspace``: a
+# captured graph then owns its own, and calls on several streams share none.  The operators record no autograd graph; each has its gradient
+# beside it.  Their smallest calls are bound by this file, not by the GPU: the checks below are written for few Python calls.
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _dtype_code(what, *ts):
-    if ts[0].dtype not in _DTYPES or any(t is not None and t.dtype != ts[0].dtype for t in ts):
-        raise _lib.DfsfmError(f"{what}: need fp32, bf16 or fp16 tensors of one type")
-    return _DTYPES[ts[0].dtype]
+def _on_first_device(fn):
+    """``_on_device`` for operators whose first argument is a tensor: its device is made current if it is not; ``_operands`` refuses
+    tensors elsewhere."""
+    @functools.wraps(fn)
+    def wrapper(x, *args, **kw):
+        if not x.is_cuda:
+            raise _lib.DfsfmError("HIP ops need device tensors (there is no CPU path)")
+        if x.get_device() == torch.cuda.current_device():
+            return fn(x, *args, **kw)
+        with torch.cuda.device(x.get_device()):
+            return fn(x, *args, **kw)
+    return wrapper
 
 
-def _no_graph(what, *ts):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        raise _lib.DfsfmError(f"{what}: records no autograd graph: call it on detached tensors (or under torch.no_grad()) and its "
-                              "gradient with the backward function beside it")
+def _operands(what, x, same, others):
+    """The type code of x; every tensor of ``same`` has its type, and those of ``others`` too are on its device (None: absent)."""
+    code, dev = _DTYPES.get(x.dtype), x.get_device()
+    if code is None:
+        raise _lib.DfsfmError(f"{what}: need fp32, bf16 or fp16 tensors, got {x.dtype}")
+    graph = torch.is_grad_enabled()
+    for t in (x, *same, *others):
+        if t is None:
+            continue
+        if t.get_device() != dev:
+            raise _lib.DfsfmError(f"{what}: operands live on different devices, or not on a GPU")
+        if graph and t.requires_grad:
+            raise _lib.DfsfmError(f"{what}: records no autograd graph: call it on detached tensors (or under torch.no_grad()) and its "
+                                  "gradient with the backward function beside it")
+    for t in same:
+        if t is not None and t.dtype != x.dtype:
+            raise _lib.DfsfmError(f"{what}: need tensors of one type, got {x.dtype} and {t.dtype}")
+    return code
 
 
-def _norm_rows(t, what):
-    """(rows, row stride) of [..., C] rows with unit inner stride; copies what does not flatten to uniformly strided rows."""
-    if t.dim() < 1:
-        raise _lib.DfsfmError(f"{what}: need [..., C] tensors")
-    rows = 1
-    for s in t.shape[:-1]:
-        rows *= s
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        t = t.contiguous()
+def _norm_rows(t, C):
+    """(t, row stride) of [..., C] rows with unit inner stride; copies what does not flatten to uniformly strided rows."""
+    if t.is_contiguous():
+        return t, C
+    if C > 1 and t.stride(-1) != 1:
+        return t.contiguous(), C
     dims = [(s, st) for s, st in zip(t.shape[:-1], t.stride()[:-1]) if s != 1]
     if any(dims[i][1] != dims[i + 1][0] * dims[i + 1][1] for i in range(len(dims) - 1)):
-        t = t.contiguous()
-        return t, rows, t.shape[-1]
-    return t, rows, dims[-1][1] if dims else t.shape[-1]
+        return t.contiguous(), C
+    return t, dims[-1][1] if dims else C
 
 
-def _norm_affine(what, t, C, *ws):
-    """`wtype` of gamma / beta: the rows' type or fp32, [C], dense."""
-    for w in ws:
-        if w.shape != (C,) or w.dtype != ws[0].dtype or w.dtype not in (t.dtype, torch.float32):
-            raise _lib.DfsfmError(f"{what}: gamma and beta are [C] of one type, the rows' or fp32")
-    return [w.contiguous() for w in ws], _DTYPES[ws[0].dtype]
+def _norm_affine(what, x, C, w):
+    if w.shape != (C,) or (w.dtype != x.dtype and w.dtype != torch.float32):
+        raise _lib.DfsfmError(f"{what}: gamma and beta are [C] of one type, the rows' or fp32")
+    return w if w.is_contiguous() else w.contiguous()
 
 
-@_on_device
+@_on_first_device
 def layernorm_forward(x, gamma, beta, eps=1e-5, residual=None):
     """(x - mean) / sqrt(var + eps) * gamma + beta (+ residual) over the last dim of x [..., C], fp32 / bf16 / fp16, C up to 16384; gamma
     and beta [C] in x's type or fp32.  Returns (y dense in x's type, mean [...], rstd [...] in fp32): what ``layernorm_backward`` reads."""
-    _require_cuda(x, gamma, beta, residual)
-    _no_graph("layernorm_forward", x, gamma, beta, residual)
-    code = _dtype_code("layernorm_forward", x, residual)
-    x, rows, ldx = _norm_rows(x, "layernorm_forward")
-    C = x.shape[-1]
-    (gamma, beta), wtype = _norm_affine("layernorm_forward", x, C, gamma, beta)
-    ldr = 0
+    code = _operands("layernorm_forward", x, (residual,), (gamma, beta))
+    if x.dim() < 1:
+        raise _lib.DfsfmError("layernorm_forward: need [..., C] tensors")
+    shape = x.shape
+    C = shape[-1]
+    if C == 0 or C > 16384 or gamma.dtype != beta.dtype:
+        raise _lib.DfsfmError("layernorm_forward: rows of 1 to 16384 channels, gamma and beta of one type")
+    gamma, beta = _norm_affine("layernorm_forward", x, C, gamma), _norm_affine("layernorm_forward", x, C, beta)
+    x, ldx = _norm_rows(x, C)
+    rp, ldr = None, 0
     if residual is not None:
-        if residual.shape != x.shape:
+        if residual.shape != shape:
             raise _lib.DfsfmError("layernorm_forward: the residual has x's shape")
-        residual, _, ldr = _norm_rows(residual, "layernorm_forward")
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean, rstd = torch.empty((2, *x.shape[:-1]), dtype=torch.float32, device=x.device).unbind(0)
-    rc = _lib.lib().dfsfm_layernorm_forward(x.data_ptr(), ldx, gamma.data_ptr(), beta.data_ptr(), wtype, float(eps),
-                                            None if residual is None else residual.data_ptr(), ldr, y.data_ptr(), mean.data_ptr(),
-                                            rstd.data_ptr(), rows, C, code, _stream())
-    _lib.check(rc, "dfsfm_layernorm_forward")
+        residual, ldr = _norm_rows(residual, C)
+        rp = residual.data_ptr()
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    mean, rstd = x.new_empty(shape[:-1], dtype=torch.float32), x.new_empty(shape[:-1], dtype=torch.float32)
+    rc = _lib.lib().dfsfm_layernorm_forward(x.data_ptr(), ldx, gamma.data_ptr(), beta.data_ptr(), _DTYPES[gamma.dtype], eps, rp, ldr,
+                                            y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), x.numel() // C, C, code,
+                                            _raw_stream(x.get_device()))
+    if rc:
+        _lib.check(rc, "dfsfm_layernorm_forward")
     return y, mean, rstd
 
 
-@_on_device
+@_on_first_device
 def layernorm_backward(dy, x, mean, rstd, gamma, need_weights=True):
     """Gradients of ``layernorm_forward`` for dy [..., C]: (dx in x's type, dgamma, dbeta in gamma's type; the two are None without
     ``need_weights``).  The residual's gradient is dy.  Sums over the rows run in a fixed order: the same call gives the same bits."""
-    _require_cuda(dy, x, mean, rstd, gamma)
-    _no_graph("layernorm_backward", dy, x, gamma)
-    code = _dtype_code("layernorm_backward", x, dy)
-    if dy.shape != x.shape:
-        raise _lib.DfsfmError("layernorm_backward: dy has x's shape")
+    code = _operands("layernorm_backward", x, (dy,), (mean, rstd, gamma))
     shape = x.shape
-    x, rows, ldx = _norm_rows(x, "layernorm_backward")
-    dy, _, lddy = _norm_rows(dy, "layernorm_backward")
+    if x.dim() < 1 or dy.shape != shape:
+        raise _lib.DfsfmError("layernorm_backward: dy has x's shape [..., C]")
     C = shape[-1]
-    (gamma,), wtype = _norm_affine("layernorm_backward", x, C, gamma)
-    for t in (mean, rstd):
-        if t.dtype != torch.float32 or t.shape != shape[:-1]:
-            raise _lib.DfsfmError("layernorm_backward: mean and rstd are what layernorm_forward returned for x")
+    if C == 0 or C > 16384:
+        raise _lib.DfsfmError("layernorm_backward: rows of 1 to 16384 channels")
+    gamma = _norm_affine("layernorm_backward", x, C, gamma)
+    if mean.dtype != torch.float32 or rstd.dtype != torch.float32 or mean.shape != shape[:-1] or rstd.shape != shape[:-1]:
+        raise _lib.DfsfmError("layernorm_backward: mean and rstd are what layernorm_forward returned for x")
     mean, rstd = mean.contiguous(), rstd.contiguous()
+    x, ldx = _norm_rows(x, C)
+    dy, lddy = _norm_rows(dy, C)
+    rows = x.numel() // C
     L = _lib.lib()
-    dx = torch.empty(shape, dtype=x.dtype, device=x.device)
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     dg = db = ws = None
     nbytes = 0
     if need_weights:
-        dg, db = torch.empty((2, C), dtype=gamma.dtype, device=x.device).unbind(0)
+        dg, db = torch.empty_like(gamma), torch.empty_like(gamma)
         nbytes = L.dfsfm_layernorm_backward_workspace(rows, C, code)
-        ws = torch.empty((nbytes,), dtype=torch.uint8, device=x.device)
-    rc = L.dfsfm_layernorm_backward(dy.data_ptr(), lddy, x.data_ptr(), ldx, mean.data_ptr(), rstd.data_ptr(), gamma.data_ptr(), wtype,
-                                    dx.data_ptr(), None if dg is None else dg.data_ptr(), None if db is None else db.data_ptr(), rows, C,
-                                    code, None if ws is None else ws.data_ptr(), nbytes, _stream())
-    _lib.check(rc, "dfsfm_layernorm_backward")
+        ws = x.new_empty(nbytes, dtype=torch.uint8)
+    rc = L.dfsfm_layernorm_backward(dy.data_ptr(), lddy, x.data_ptr(), ldx, mean.data_ptr(), rstd.data_ptr(), gamma.data_ptr(),
+                                    _DTYPES[gamma.dtype], dx.data_ptr(), None if dg is None else dg.data_ptr(),
+                                    None if db is None else db.data_ptr(), rows, C, code, None if ws is None else ws.data_ptr(), nbytes,
+                                    _raw_stream(x.get_device()))
+    if rc:
+        _lib.check(rc, "dfsfm_layernorm_backward")
     return dx, dg, db
 
 
@@ -1770,83 +1795,101 @@ def rotary_frequencies(rotated, base=10000.0, axes=1, scaling="none", factor=1.0
 
 
 def _rotary(what, x, positions, inv_freq, amplitude, axes, interleaved, inplace, backward):
-    _require_cuda(x, positions, inv_freq)
-    _no_graph(what, x)
-    code = _dtype_code(what, x)
+    code = _operands(what, x, (), (positions, inv_freq))
     if x.dim() != 4:
         raise _lib.DfsfmError(f"{what}: x is [N, L, H, D]")
     N, L, H, D = x.shape
-    if axes not in (1, 2) or inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not 0 < 2 * axes * inv_freq.numel() <= D:
+    pairs = inv_freq.numel()
+    if axes not in (1, 2) or inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not 0 < 2 * axes * pairs <= D:
         raise _lib.DfsfmError(f"{what}: inv_freq is fp64 [pairs] with 2 * axes * pairs <= D, axes 1 or 2")
-    if positions.dtype not in (torch.int32, torch.int64):
-        raise _lib.DfsfmError(f"{what}: positions are int32 or int64")
-    want = (N, L) if axes == 1 else (N, L, axes)
+    if D > 512 or H > 65535 or N * L >= 1 << 31:
+        raise _lib.DfsfmError(f"{what}: up to 512 channels, 65535 heads, 2^31 tokens")
+    want = (N, L) if axes == 1 else (N, L, 2)
     if positions.shape != want and positions.shape != want[1:]:
         raise _lib.DfsfmError(f"{what}: positions are {list(want[1:])} or {list(want)}")
-    positions = positions.to(torch.int64).expand(want)
-    if axes == 1:
-        positions = positions[..., None]
-    inv_freq = inv_freq.contiguous()
+    if positions.dtype != torch.int64:
+        if positions.dtype != torch.int32:
+            raise _lib.DfsfmError(f"{what}: positions are int32 or int64")
+        positions = positions.to(torch.int64)
+    ps = positions.stride()
+    if len(ps) < len(want):
+        ps = (0, *ps)                           # one set of positions for the whole batch
+    if not inv_freq.is_contiguous():
+        inv_freq = inv_freq.contiguous()
+    xs = x.stride()
     if inplace:
-        at = 1                              # every element has its own place: strides of the sizes over 1 nest, the smallest first
-        for st, size in sorted((x.stride(i), x.shape[i]) for i in range(4) if x.shape[i] > 1):
+        at = 1                                  # every element has its own place: strides nest, the smallest first
+        for st, size in sorted((st, size) for st, size in zip(xs, x.shape) if size > 1):
             if st < at:
                 raise _lib.DfsfmError(f"{what}: in-place tensors may not overlap themselves")
             at = st * size
-        if D > 1 and x.stride(3) != 1:
+        if D > 1 and xs[3] != 1:
             raise _lib.DfsfmError(f"{what}: in-place tensors need a unit channel stride")
-        y = x
+        y, ys = x, xs
     else:
-        if D > 1 and x.stride(3) != 1:
+        if D > 1 and xs[3] != 1:
             x = x.contiguous()
-        y = torch.empty((N, L, H, D), dtype=x.dtype, device=x.device)
-    rc = _lib.lib().dfsfm_rotary(x.data_ptr(), x.stride(0), x.stride(1), x.stride(2), y.data_ptr(), y.stride(0), y.stride(1), y.stride(2),
-                                 positions.data_ptr(), positions.stride(0), positions.stride(1), positions.stride(2), inv_freq.data_ptr(),
-                                 inv_freq.numel(), axes, 1 if interleaved else 0, 1 if backward else 0, float(amplitude), N, L, H, D, code,
-                                 _stream())
-    _lib.check(rc, "dfsfm_rotary")
+            xs = x.stride()
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
+        ys = y.stride()
+    rc = _lib.lib().dfsfm_rotary(x.data_ptr(), xs[0], xs[1], xs[2], y.data_ptr(), ys[0], ys[1], ys[2], positions.data_ptr(), ps[0], ps[1],
+                                 0 if axes == 1 else ps[2], inv_freq.data_ptr(), pairs, axes, 1 if interleaved else 0, backward, amplitude, N,
+                                 L, H, D, code, _raw_stream(x.get_device()))
+    if rc:
+        _lib.check(rc, "dfsfm_rotary")
     return y
 
 
-@_on_device
+@_on_first_device
 def rotary(x, positions, inv_freq, amplitude=1.0, axes=1, interleaved=False, inplace=False):
     """Rotary positions of the heads x [N, L, H, D] (fp32 / bf16 / fp16, strided views OK): each pair of channels turns by position *
     inv_freq and is scaled by ``amplitude`` (``rotary_frequencies`` makes both).  positions [L] or [N, L], any sign; with ``axes`` = 2
     (row and column of image tokens) [L, 2] or [N, L, 2], one section of 2 * pairs channels an axis.  Pairs are (p, p + pairs) of a
     section or, ``interleaved``, (2p, 2p + 1); channels behind the sections stay.  Returns a dense tensor, or x changed ``inplace``.
     q and k that are columns of one projection turn in one call on their common view."""
-    return _rotary("rotary", x, positions, inv_freq, amplitude, axes, interleaved, inplace, False)
+    return _rotary("rotary", x, positions, inv_freq, amplitude, axes, interleaved, inplace, 0)
 
 
-@_on_device
+@_on_first_device
 def rotary_backward(dy, positions, inv_freq, amplitude=1.0, axes=1, interleaved=False, inplace=False):
     """Gradient of ``rotary`` for its result's gradient dy: the same turn the other way."""
-    return _rotary("rotary_backward", dy, positions, inv_freq, amplitude, axes, interleaved, inplace, True)
+    return _rotary("rotary_backward", dy, positions, inv_freq, amplitude, axes, interleaved, inplace, 1)
 
 
-def _attention_args(what, q, k, v, kv_lens, kv_mask, scale):
-    """Checked tensors of a cross attention call: (q, k, v, lens int32, mask uint8, scale, sizes, dtype code)."""
-    _require_cuda(q, k, v, kv_lens, kv_mask)
-    code = _dtype_code(what, q, k, v)
-    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+def _attention_args(what, q, k, v, kv_lens, kv_mask, scale, more=()):
+    """Checked tensors of a cross attention call: (q, k, v, pointers of kv_lens and kv_mask, what holds them, scale, sizes, type code)."""
+    code = _operands(what, q, (k, v, *more), (kv_lens, kv_mask))
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
         raise _lib.DfsfmError(f"{what}: need q [N, L, H, D] and k, v [N, S, Hkv, D]")
-    (N, L, H, D), (S, Hkv) = q.shape, k.shape[1:3]
+    (N, L, H, D), (Nk, S, Hkv, Dk) = q.shape, k.shape
+    if Nk != N or Dk != D:
+        raise _lib.DfsfmError(f"{what}: need q [N, L, H, D] and k, v [N, S, Hkv, D]")
     if D == 0 or D > 128 or D % 8 or (H % Hkv if Hkv else H):
         raise _lib.DfsfmError(f"{what}: head dims are multiples of 8 up to 128, query heads a multiple of the key heads")
+    lens = mask = None
     if kv_lens is not None:
         if kv_lens.shape != (N,) or kv_lens.dtype not in (torch.int32, torch.int64):
             raise _lib.DfsfmError(f"{what}: kv_lens is int32 or int64 [N]")
-        kv_lens = kv_lens.clamp(0, S).to(torch.int32) if kv_lens.dtype == torch.int64 else kv_lens
+        if kv_lens.dtype == torch.int64:
+            kv_lens = kv_lens.clamp(0, S).to(torch.int32)
         kv_lens = kv_lens.contiguous()
+        lens = kv_lens.data_ptr()
     if kv_mask is not None:
         if kv_mask.shape != (N, S):
             raise _lib.DfsfmError(f"{what}: kv_mask is [N, S]")
         kv_mask = _as_u8(kv_mask)
-    scale = D ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
+        mask = kv_mask.data_ptr()
+    if scale is None:
+        scale = D ** -0.5
+    elif not 0.0 < scale < float("inf"):
         raise _lib.DfsfmError(f"{what}: the scale is positive")
-    q, k, v = (t if t.stride(3) == 1 else t.contiguous() for t in (q, k, v))
-    return q, k, v, kv_lens, kv_mask, scale, (N, L, S, H, Hkv, D), code
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    if k.stride(3) != 1:
+        k = k.contiguous()
+    if v.stride(3) != 1:
+        v = v.contiguous()
+    return q, k, v, lens, mask, (kv_lens, kv_mask), scale, (N, L, S, H, Hkv, D), code
 
 
 def _heads_ptr(t):
@@ -1854,51 +1897,51 @@ def _heads_ptr(t):
     return t.data_ptr(), s[0], s[1], s[2]
 
 
-@_on_device
+@_on_first_device
 def cross_attention(q, k, v, kv_lens=None, kv_mask=None, scale=None):
     """softmax(scale * q k^T) v of q [N, L, H, D] over states k, v [N, S, Hkv, D] of another length, fp32 / bf16 / fp16, D a multiple of 8
-    up to 128, strided views OK (unit channel stride); query heads h * H / Hkv ... share key head h.  Sequence n looks at its keys s <
+    up to 128, strided views OK (unit channel stride); query head h reads key head h // (H / Hkv).  Sequence n looks at its keys s <
     kv_lens[n] (int tensor on the device, clamped to 0 .. S) with kv_mask[n, s] true; what padded places hold, NaN included, does not
     matter, and a sequence without keys gives zeros.  ``scale`` defaults to D ** -0.5.  L = 1 is the single-token form: the keys are
     split over the chip and joined.  Returns (out [N, L, H, D] dense, lse [N, H, L] fp32: the scores' log-sum-exp, -inf without keys)."""
-    _no_graph("cross_attention", q, k, v)
-    q, k, v, kv_lens, kv_mask, scale, sizes, code = _attention_args("cross_attention", q, k, v, kv_lens, kv_mask, scale)
+    q, k, v, lens, mask, hold, scale, sizes, code = _attention_args("cross_attention", q, k, v, kv_lens, kv_mask, scale)
     N, L, S, H, Hkv, D = sizes
-    out = torch.empty((N, L, H, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((N, H, L), dtype=torch.float32, device=q.device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = q.new_empty((N, H, L), dtype=torch.float32)
     lib = _lib.lib()
-    nbytes = lib.dfsfm_cross_attention_workspace(*sizes)
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=q.device) if nbytes else None
-    rc = lib.dfsfm_cross_attention(*_heads_ptr(q), *_heads_ptr(k), *_heads_ptr(v), None if kv_lens is None else kv_lens.data_ptr(),
-                                   None if kv_mask is None else kv_mask.data_ptr(), out.data_ptr(), lse.data_ptr(), *sizes, scale, code,
-                                   None if ws is None else ws.data_ptr(), nbytes, _stream())
-    _lib.check(rc, "dfsfm_cross_attention")
+    nbytes = lib.dfsfm_cross_attention_workspace(N, L, S, H, Hkv, D)
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    rc = lib.dfsfm_cross_attention(*_heads_ptr(q), *_heads_ptr(k), *_heads_ptr(v), lens, mask, out.data_ptr(), lse.data_ptr(), N, L, S, H, Hkv,
+                                   D, scale, code, ws.data_ptr() if nbytes else None, nbytes, _raw_stream(q.get_device()))
+    if rc:
+        _lib.check(rc, "dfsfm_cross_attention")
     return out, lse
 
 
-@_on_device
+@_on_first_device
 def cross_attention_backward(dout, q, k, v, out, lse, kv_lens=None, kv_mask=None, scale=None):
     """Gradients (dq, dk, dv), dense, of ``cross_attention`` for dout [N, L, H, D]; out and lse are what it returned, the other arguments
     what it was called with.  Keys that are not there get zeros.  Sums run in a fixed order: the same call gives the same bits.
     fp16: products p * ds are carried with a power of two per column, so gradients far below fp16's normal range keep their digits."""
-    _no_graph("cross_attention_backward", dout, q, k, v)
-    q, k, v, kv_lens, kv_mask, scale, sizes, code = _attention_args("cross_attention_backward", q, k, v, kv_lens, kv_mask, scale)
-    _require_cuda(dout, out, lse)
+    q, k, v, lens, mask, hold, scale, sizes, code = _attention_args("cross_attention_backward", q, k, v, kv_lens, kv_mask, scale, (dout, out))
     N, L, S, H, Hkv, D = sizes
-    if _dtype_code("cross_attention_backward", q, dout, out) != code or dout.shape != q.shape or out.shape != q.shape:
+    if dout.shape != q.shape or out.shape != q.shape:
         raise _lib.DfsfmError("cross_attention_backward: dout and out have q's shape and type")
-    if lse.shape != (N, H, L) or lse.dtype != torch.float32:
+    if lse.shape != (N, H, L) or lse.dtype != torch.float32 or lse.get_device() != q.get_device():
         raise _lib.DfsfmError("cross_attention_backward: lse is what cross_attention returned, fp32 [N, H, L]")
-    dout, out, lse = (t if t.stride(-1) == 1 else t.contiguous() for t in (dout, out, lse))
+    if dout.stride(3) != 1:
+        dout = dout.contiguous()
+    if out.stride(3) != 1:
+        out = out.contiguous()
     lse = lse.contiguous()
-    dq = torch.empty((N, L, H, D), dtype=q.dtype, device=q.device)
-    dk, dv = (torch.empty((N, S, Hkv, D), dtype=q.dtype, device=q.device) for _ in range(2))
+    dq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    dk, dv = torch.empty_like(k, memory_format=torch.contiguous_format), torch.empty_like(v, memory_format=torch.contiguous_format)
     lib = _lib.lib()
-    nbytes = lib.dfsfm_cross_attention_backward_workspace(*sizes)
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=q.device)
+    nbytes = lib.dfsfm_cross_attention_backward_workspace(N, L, S, H, Hkv, D)
+    ws = q.new_empty(nbytes, dtype=torch.uint8)
     rc = lib.dfsfm_cross_attention_backward(*_heads_ptr(dout), *_heads_ptr(q), *_heads_ptr(k), *_heads_ptr(v), *_heads_ptr(out),
-                                            lse.data_ptr(), None if kv_lens is None else kv_lens.data_ptr(),
-                                            None if kv_mask is None else kv_mask.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                                            *sizes, scale, code, ws.data_ptr(), nbytes, _stream())
-    _lib.check(rc, "dfsfm_cross_attention_backward")
+                                            lse.data_ptr(), lens, mask, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), N, L, S, H, Hkv, D, scale,
+                                            code, ws.data_ptr(), nbytes, _raw_stream(q.get_device()))
+    if rc:
+        _lib.check(rc, "dfsfm_cross_attention_backward")
     return dq, dk, dv
