@@ -114,6 +114,11 @@ __device__ __forceinline__ Frag<T> pack8(const f32x16& s, int t) {
     return f;
 }
 
+// Waves a SIMD that the forward and dq kernels are compiled for: two (256 registers a wave), so that one wave's exponentials run beside the
+// other's products.  fp32 at D = 128 holds twice the operands and would spill.
+template <typename T, int DP>
+constexpr int WAVES = sizeof(T) == 4 && DP == 128 ? 1 : 2;
+
 struct Tensor {
     const void* p;
     int64_t n, l, h;                       // element strides of [N, length, heads, D]; the channel stride is 1
@@ -132,42 +137,56 @@ struct Attn {
     float scale;
 };
 
-// What a workgroup works on: grid.x = (splits, tiles, N * kv heads), heads fastest.
+// What a workgroup works on: grid.x = (splits, N * kv heads, tiles), tiles fastest: neighbours in time are tiles of one head, spread over all
+// XCDs, so sequences of unequal lengths load the chip evenly.  Heads fastest (a head's tiles on one XCD's L2) left XCDs with short sequences
+// idle: 1.11 ms against 0.82 for the forward pass of 4 x 4800 x 6400 (ragged) x 16 heads x 128.
 struct Job {
     int n, hk, tile, split;
     __device__ __forceinline__ Job(const Attn& a) {
         const int hkv = a.H / a.G, heads = a.N * hkv;
-        const int head = blockIdx.x % heads, rest = blockIdx.x / heads;
+        tile = blockIdx.x % a.tiles;
+        const int rest = blockIdx.x / a.tiles, head = rest % heads;
+        split = rest / heads;
         n = head / hkv;
         hk = head % hkv;
-        tile = rest % a.tiles;
-        split = rest / a.tiles;
     }
 };
 
 __device__ __forceinline__ int valid_len(const Attn& a, int n) { return a.lens ? min(max(a.lens[n], 0), a.S) : a.S; }
 
-// A tile of 64 rows x DP channels on its way from memory through the registers of 256 threads into LDS.
+// A tile of 64 rows x DP channels on its way from memory through the registers of 256 threads into LDS.  A thread's 32-bit byte offsets
+// within a tile are the same for every whole tile: the address costs one scalar base a tile and no vector arithmetic.
 template <typename T, int DP>
 struct Stage {
     static constexpr int VPR = DP / 8, PER = KT * VPR / 256;
     Frag<T> r[PER];
-    // row: maps a tile row to its address
-    template <typename F>
-    __device__ __forceinline__ void load(F row, int D) {
+    unsigned off[PER];
+    unsigned stride;                       // bytes a row
+    int D;
+    __device__ __forceinline__ Stage(int64_t stride_, int D_) : stride((unsigned)(stride_ * sizeof(T))), D(D_) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) off[i] = offset(i, KT - 1);
+    }
+    __device__ __forceinline__ unsigned offset(int i, int last) const {
+        const int e = threadIdx.x + 256 * i;
+        return min(e / VPR, last) * stride + e % VPR * 8 * (unsigned)sizeof(T);
+    }
+    // rows base .. base + rows - 1, the last one again behind them
+    __device__ __forceinline__ void load(const T* base, int rows) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int e = threadIdx.x + 256 * i, c = e % VPR * 8;
-            r[i] = c < D ? load8<T>(row(e / VPR) + c) : zero_frag<T>();
+            const unsigned o = rows >= KT ? off[i] : offset(i, rows - 1);
+            const T* p = reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + o);
+            r[i] = (threadIdx.x + 256 * i) % VPR * 8 < D ? load8<T>(p) : zero_frag<T>();
         }
     }
     // rows whose bit in `keep` is 0 become zeros
     __device__ __forceinline__ void store(T* tile, int pitch, unsigned long long keep) const {
+        typedef Frag<T> at16 __attribute__((aligned(16)));
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int e = threadIdx.x + 256 * i, row = e / VPR, c = e % VPR * 8;
-            typedef Frag<T> at16 __attribute__((aligned(16)));
-            *reinterpret_cast<at16*>(tile + row * pitch + c) = keep >> row & 1 ? r[i] : zero_frag<T>();
+            *reinterpret_cast<at16*>(tile + row * pitch + c) = ~keep == 0 || keep >> row & 1 ? r[i] : zero_frag<T>();
         }
     }
 };
@@ -264,7 +283,7 @@ struct ColumnScale {
 // ---------------------------------------------------------------- forward
 // 4 waves x 32 rows a workgroup; tiles of 64 keys, two in LDS.
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void attn_forward_kernel(const Attn a) {
+__global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_forward_kernel(const Attn a) {
     constexpr int KP = PITCH<T, DP>, VP = PITCH_T<T, DP>, DB = DP / 32, KS = DP / 16;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* ks = reinterpret_cast<T*>(smem);
@@ -287,10 +306,10 @@ __global__ __launch_bounds__(256) void attn_forward_kernel(const Attn a) {
     }
     const T* kb = static_cast<const T*>(a.k.p) + job.n * a.k.n + job.hk * a.k.h;
     const T* vb = static_cast<const T*>(a.v.p) + job.n * a.v.n + job.hk * a.v.h;
-    Stage<T, DP> sk, sv;
+    Stage<T, DP> sk(a.k.l, a.D), sv(a.v.l, a.D);
     auto fetch = [&](int s0) {
-        sk.load([&](int row) { return kb + (int64_t)min(s0 + row, end - 1) * a.k.l; }, a.D);
-        sv.load([&](int row) { return vb + (int64_t)min(s0 + row, end - 1) * a.v.l; }, a.D);
+        sk.load(kb + s0 * a.k.l, end - s0);
+        sv.load(vb + s0 * a.v.l, end - s0);
     };
     f32x16 acc[DB];
 #pragma unroll
@@ -416,8 +435,13 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(const Attn a) {
 }
 
 // dq: the forward kernel's frame, K read both ways.
-template <typename T, int DP>
-__global__ __launch_bounds__(256) void attn_dq_kernel(const Attn a) {
+//
+// SHORT (up to 128 keys: both tiles stay in LDS) also computes delta, as the sum of p dp over the keys it is equal to.  The sum over the
+// channels of dout times the ROUNDED out is off by half a step of out, an error that all keys of a row share: over many keys it drowns in
+// the roundings of ds, over few it does not (dq of 4800 x 77 fp16: 3.2e-4 off in the 2-norm against 2.1e-4 that the output's rounding alone
+// costs).  Two of three products are then made twice, over two tiles at most; a pass over dout and out is saved.
+template <typename T, int DP, bool SHORT>
+__global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn a) {
     constexpr int KP = PITCH_T<T, DP>, VP = PITCH<T, DP>, DB = DP / 32, KS = DP / 16;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* ks = reinterpret_cast<T*>(smem);
@@ -441,51 +465,87 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(const Attn a) {
         of[s] = r < R && c < a.D ? load8<T>(op + c) : zero_frag<T>();
     }
     const int64_t at = ((int64_t)job.n * a.H + h) * a.L + l;
-    const float c = a.scale * LOG2E, lse = r < R ? a.lse[at] : NEG, delta = r < R ? a.delta[at] : 0.f;
+    const float c = a.scale * LOG2E, lse = r < R ? a.lse[at] : NEG;
     const float lse2 = lse == NEG ? INFINITY : lse * LOG2E;              // a row without keys has p = 0
+    float delta = !SHORT && r < R ? a.delta[at] : 0.f;
     const T* kb = static_cast<const T*>(a.k.p) + job.n * a.k.n + job.hk * a.k.h;
     const T* vb = static_cast<const T*>(a.v.p) + job.n * a.v.n + job.hk * a.v.h;
-    Stage<T, DP> sk, sv;
+    Stage<T, DP> sk(a.k.l, a.D), sv(a.v.l, a.D);
     auto fetch = [&](int s0) {
-        sk.load([&](int row) { return kb + (int64_t)min(s0 + row, end - 1) * a.k.l; }, a.D);
-        sv.load([&](int row) { return vb + (int64_t)min(s0 + row, end - 1) * a.v.l; }, a.D);
+        sk.load(kb + s0 * a.k.l, end - s0);
+        sv.load(vb + s0 * a.v.l, end - s0);
+    };
+    auto stage = [&](int s0, int buf) {
+        const unsigned long long bits = key_bits(a, job.n, s0, end);
+        sk.store(ks + buf * KT * KP, KP, bits);
+        sv.store(vs + buf * KT * VP, VP, bits);
+        if (threadIdx.x < KT) bias[buf * KT + threadIdx.x] = bits >> threadIdx.x & 1 ? 0.f : NEG;
+        return bits;
     };
     f32x16 acc[DB];
 #pragma unroll
     for (int b = 0; b < DB; ++b) acc[b] = splat16(0.f);
     ColumnScale<T, DB> cs;
-    if (beg < end) fetch(beg);
-    int buf = 0;
-    for (int s0 = beg; s0 < end; s0 += KT, buf ^= 1) {
-        const unsigned long long bits = key_bits(a, job.n, s0, end);
-        T* kt = ks + buf * KT * KP;
-        T* vt = vs + buf * KT * VP;
-        float* bt = bias + buf * KT;
-        sk.store(kt, KP, bits);
-        sv.store(vt, VP, bits);
-        if (threadIdx.x < KT) bt[threadIdx.x] = bits >> threadIdx.x & 1 ? 0.f : NEG;
-        __syncthreads();
-        if (s0 + KT < end) fetch(s0 + KT);
-        if (bits == 0) continue;
+    // p dp of 32 keys, dp less delta
+    auto products = [&](int buf, int b, bool whole, f32x16& ds) {
+        const T* kt = ks + buf * KT * KP;
+        const T* vt = vs + buf * KT * VP;
+        f32x16 st = whole ? splat16(0.f) : rows16(bias + buf * KT + 32 * b, lane);
+        ds = splat16(-delta);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            st = Mma<T>::run(read_rows(kt, KP, 32 * b, 16 * s, lane), qf[s], st);
+            ds = Mma<T>::run(read_rows(vt, VP, 32 * b, 16 * s, lane), of[s], ds);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) ds[j] *= __builtin_amdgcn_exp2f(fmaf(st[j], c, -lse2));
+    };
+    auto accumulate = [&](int buf, bool whole) {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            f32x16 st = ~bits ? rows16(bt + 32 * b, lane) : splat16(0.f);
             f32x16 ds[1];
-            ds[0] = splat16(-delta);
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                st = Mma<T>::run(read_rows(kt, KP, 32 * b, 16 * s, lane), qf[s], st);
-                ds[0] = Mma<T>::run(read_rows(vt, VP, 32 * b, 16 * s, lane), of[s], ds[0]);
-            }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) ds[0][j] *= __builtin_amdgcn_exp2f(fmaf(st[j], c, -lse2));
+            products(buf, b, whole, ds[0]);
             cs.apply(ds, acc);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const Frag<T> p = pack8<T>(ds[0], u);
 #pragma unroll
-                for (int d = 0; d < DB; ++d) acc[d] = Mma<T>::run(read_cols(kt, KP, 32 * b + 16 * u, 32 * d, lane), p, acc[d]);
+                for (int d = 0; d < DB; ++d)
+                    acc[d] = Mma<T>::run(read_cols(ks + buf * KT * KP, KP, 32 * b + 16 * u, 32 * d, lane), p, acc[d]);
             }
+        }
+    };
+    if (beg < end) fetch(beg);
+    if constexpr (SHORT) {
+        unsigned long long bits[2] = {0, 0};
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+            if (t * KT < end) {
+                bits[t] = stage(t * KT, t);
+                if (t == 0 && KT < end) fetch(KT);
+            }
+        __syncthreads();
+        float sum = 0.f;
+        for (int t = 0; t * KT < end; ++t)
+            if (bits[t]) {
+                for (int b = 0; b < 2; ++b) {
+                    f32x16 ds;
+                    products(t, b, ~bits[t] == 0, ds);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) sum += ds[j];
+                }
+            }
+        delta = dfsfm::add_xor32(sum);
+        if (r < R && lane < 32) a.delta[at] = delta;
+        for (int t = 0; t * KT < end; ++t)
+            if (bits[t]) accumulate(t, ~bits[t] == 0);
+    } else {
+        int buf = 0;
+        for (int s0 = beg; s0 < end; s0 += KT, buf ^= 1) {
+            const unsigned long long bits = stage(s0, buf);
+            __syncthreads();
+            if (s0 + KT < end) fetch(s0 + KT);
+            if (bits) accumulate(buf, ~bits == 0);
         }
     }
     if (r >= R) return;
@@ -509,12 +569,13 @@ __global__ __launch_bounds__(256) void attn_dkdv_kernel(const Attn a) {
     float* rowv = reinterpret_cast<float*>(os + 2 * KT * P);              // [2][2][64]: -lse / scale, -delta
     const Job job(a);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hkv = a.H / a.G;
-    const int R = a.L * a.G, s = job.tile * 128 + wave * 32 + (lane & 31);
+    const int s = job.tile * 128 + wave * 32 + (lane & 31);
     const int len = valid_len(a, job.n);
     bool there = s < len;
     if (a.mask) there = there && a.mask[(int64_t)job.n * a.S + min(s, a.S - 1)] != 0;
-    const int per = ((R + KT - 1) / KT + a.splits - 1) / a.splits * KT;
-    const int beg = min(R, job.split * per), end = min(R, beg + per);
+    // a tile is 64 queries of one of the G heads; splits take whole tiles
+    const int lt = (a.L + KT - 1) / KT, per = (lt * a.G + a.splits - 1) / a.splits;
+    const int beg = min(lt * a.G, job.split * per), end = min(lt * a.G, beg + per);
 
     Frag<T> kf[KS], vf[KS];
     const T* kp = static_cast<const T*>(a.k.p) + job.n * a.k.n + (int64_t)min(s, a.S - 1) * a.k.l + job.hk * a.k.h;
@@ -528,17 +589,20 @@ __global__ __launch_bounds__(256) void attn_dkdv_kernel(const Attn a) {
     const T* qb = static_cast<const T*>(a.q.p) + job.n * a.q.n + job.hk * a.G * a.q.h;
     const T* ob = static_cast<const T*>(a.dout.p) + job.n * a.dout.n + job.hk * a.G * a.dout.h;
     const int64_t vec = ((int64_t)job.n * a.H + job.hk * a.G) * a.L;
-    Stage<T, DP> sq, so;
+    Stage<T, DP> sq(a.q.l, a.D), so(a.dout.l, a.D);
     float rv = 0.f;                         // threads 0..63: -lse / scale of a row, 64..127: -delta
-    auto fetch = [&](int r0) {
-        sq.load([&](int row) { const int r = min(r0 + row, end - 1); return qb + (int64_t)(r / a.G) * a.q.l + r % a.G * a.q.h; }, a.D);
-        so.load([&](int row) { const int r = min(r0 + row, end - 1); return ob + (int64_t)(r / a.G) * a.dout.l + r % a.G * a.dout.h; }, a.D);
+    int rows = 0;                           // rows of the tile in flight
+    auto fetch = [&](int it) {
+        const int g = it / lt, l0 = (it - g * lt) * KT;
+        rows = a.L - l0;
+        sq.load(qb + g * a.q.h + l0 * a.q.l, rows);
+        so.load(ob + g * a.dout.h + l0 * a.dout.l, rows);
         if (threadIdx.x < 128) {
-            const int r = r0 + (threadIdx.x & 63);
-            const int64_t at = vec + (int64_t)(min(r, end - 1) % a.G) * a.L + min(r, end - 1) / a.G;
+            const int row = threadIdx.x & 63;
+            const int64_t at = vec + (int64_t)g * a.L + l0 + min(row, rows - 1);
             const float t = threadIdx.x < 64 ? a.lse[at] : a.delta[at];
             // a row without keys, or behind the last: a score of -inf, p = 0
-            rv = threadIdx.x < 64 ? (r < end && t != NEG ? -t / a.scale : NEG) : (r < end ? -t : 0.f);
+            rv = threadIdx.x < 64 ? (row < rows && t != NEG ? -t / a.scale : NEG) : (row < rows ? -t : 0.f);
         }
     };
     f32x16 dk[DB], dv[DB];
@@ -549,16 +613,16 @@ __global__ __launch_bounds__(256) void attn_dkdv_kernel(const Attn a) {
     const bool any = __syncthreads_or(there);
     if (any && beg < end) fetch(beg);
     int buf = 0;
-    for (int r0 = beg; any && r0 < end; r0 += KT, buf ^= 1) {
+    for (int it = beg; any && it < end; ++it, buf ^= 1) {
         T* qt = qs + buf * KT * P;
         T* ot = os + buf * KT * P;
         float* vt = rowv + buf * 128;
-        const unsigned long long keep = end - r0 >= KT ? ~0ull : (1ull << (end - r0)) - 1;
+        const unsigned long long keep = rows >= KT ? ~0ull : (1ull << rows) - 1;
         sq.store(qt, P, keep);
         so.store(ot, P, keep);
         if (threadIdx.x < 128) vt[threadIdx.x] = rv;
         __syncthreads();
-        if (r0 + KT < end) fetch(r0 + KT);
+        if (it + 1 < end) fetch(it + 1);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             f32x16 st = rows16(vt + 32 * b, lane);
@@ -620,12 +684,24 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(const float* __restrict__
 // ---------------------------------------------------------------- host
 int pad_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
-// Splits of the long axis (`length` rows of it) so that 512 workgroups (two a CU) run, 256 rows a split at least.
+// offsets within a tile of 64 rows are 32-bit byte offsets
+bool stride_ok(int64_t l) { return l >= 0 && l < (1ll << 23); }
+
+// Splits of the long axis (`length` rows of it, 256 a split at least).  512 workgroups run at a time (two a CU); as long as they number less
+// than eight such rounds the last one's idle places count, and the smallest number of splits that fills 85 % of the places is taken: 608
+// workgroups of the forward pass 2 x 4800 x 10816 x 8 x 32 fp32 take 1.21 ms, three splits of each 0.98 with the join.
 int choose_splits(int64_t groups, int64_t length) {
-    if (groups <= 0 || groups >= 512) return 1;
-    const int64_t want = (512 + groups - 1) / groups, most = (length + 255) / 256;
-    const int64_t s = want < most ? want : most;
-    return (int)(s < 1 ? 1 : s > 256 ? 256 : s);
+    if (groups <= 0 || groups >= 4096) return 1;
+    const int64_t most = length / 256 < 256 ? length / 256 : 256;
+    int best = 1;
+    double fill = 0;
+    for (int s = 1; s <= most || s == 1; ++s) {
+        const int64_t n = groups * s, places = (n + 511) / 512 * 512;
+        const double f = (double)n / (double)places;
+        if (f > fill + 0.02) fill = f, best = s;
+        if (fill >= 0.85) break;
+    }
+    return best;
 }
 
 struct Plan {
@@ -669,15 +745,23 @@ template <typename T, int DP>
 int backward_dp(Attn a, const Plan& p, T* dq, T* dk, T* dv, float* part, hipStream_t st) {
     const int64_t rows = (int64_t)a.N * a.L * a.H, nq = rows * a.D, nk = (int64_t)a.N * a.S * (a.H / a.G) * a.D;
     if (rows > 0) {
-        hipLaunchKernelGGL((attn_delta_kernel<T>), dim3((unsigned)((rows + 31) / 32)), dim3(256), 0, st, a);
         constexpr int smem = 2 * KT * (PITCH<T, DP> + PITCH_T<T, DP>) * sizeof(T) + 2 * KT * 4;
-        static dfsfm::SmemAttr attr;
-        attr.ensure(reinterpret_cast<const void*>(&attn_dq_kernel<T, DP>), smem);
+        const bool few = a.S <= 2 * KT;        // one split: choose_splits cuts from 256 keys up
         a.tiles = p.tq;
         a.splits = p.dq;
         a.numel = nq;
         a.o[0] = p.dq > 1 ? static_cast<void*>(part) : dq;
-        hipLaunchKernelGGL((attn_dq_kernel<T, DP>), dim3((unsigned)(p.heads * p.tq * p.dq)), dim3(256), smem, st, a);
+        const dim3 grid((unsigned)(p.heads * p.tq * p.dq));
+        if (few) {
+            static dfsfm::SmemAttr attr;
+            attr.ensure(reinterpret_cast<const void*>(&attn_dq_kernel<T, DP, true>), smem);
+            hipLaunchKernelGGL((attn_dq_kernel<T, DP, true>), grid, dim3(256), smem, st, a);
+        } else {
+            static dfsfm::SmemAttr attr;
+            attr.ensure(reinterpret_cast<const void*>(&attn_dq_kernel<T, DP, false>), smem);
+            hipLaunchKernelGGL((attn_delta_kernel<T>), dim3((unsigned)((rows + 31) / 32)), dim3(256), 0, st, a);
+            hipLaunchKernelGGL((attn_dq_kernel<T, DP, false>), grid, dim3(256), smem, st, a);
+        }
         if (p.dq > 1)
             hipLaunchKernelGGL((attn_sum_kernel<T>), dim3((unsigned)((nq / 4 + 255) / 256)), dim3(256), 0, st, part, nq, p.dq, dq);
     }
@@ -729,6 +813,7 @@ extern "C" int dfsfm_cross_attention(const void* q, int64_t qn, int64_t ql, int6
     if (N == 0 || L == 0 || H == 0) return DFSFM_OK;
     if (!q || !out || !lse || (S > 0 && (!k || !v)) || N < 0 || L < 0 || S < 0 || H < 0 || !(scale > 0.f)) return DFSFM_E_BADARG;
     if (!shape_ok(N, L, S, H, Hkv, D)) return DFSFM_E_UNSUPPORTED;
+    if (!stride_ok(ks) || !stride_ok(vs)) return DFSFM_E_UNSUPPORTED;
     if (workspace_bytes < dfsfm_cross_attention_workspace(N, L, S, H, Hkv, D)) return DFSFM_E_WORKSPACE;
     Attn a{};
     a.q = {q, qn, ql, qh};
@@ -767,6 +852,7 @@ extern "C" int dfsfm_cross_attention_backward(const void* dout, int64_t gn, int6
     if (N < 0 || L < 0 || S < 0 || H < 0 || !(scale > 0.f)) return DFSFM_E_BADARG;
     if ((L > 0 && (!dout || !q || !out || !lse || !dq)) || (S > 0 && (!k || !v || !dk || !dv))) return DFSFM_E_BADARG;
     if (!shape_ok(N, L, S, H, Hkv, D)) return DFSFM_E_UNSUPPORTED;
+    if (!stride_ok(ks) || !stride_ok(vs) || !stride_ok(ql) || !stride_ok(gl)) return DFSFM_E_UNSUPPORTED;
     if (workspace_bytes < dfsfm_cross_attention_backward_workspace(N, L, S, H, Hkv, D)) return DFSFM_E_WORKSPACE;
     Attn a{};
     a.q = {q, qn, ql, qh};

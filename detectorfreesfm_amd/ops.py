@@ -1856,6 +1856,12 @@ def rotary_backward(dy, positions, inv_freq, amplitude=1.0, axes=1, interleaved=
     return _rotary("rotary_backward", dy, positions, inv_freq, amplitude, axes, interleaved, inplace, 1)
 
 
+def _heads(t):
+    """[N, L, H, D] heads as the kernels read them: a unit channel stride, tokens less than 2^23 elements apart."""
+    s = t.stride()
+    return t if s[3] == 1 and s[1] < 1 << 23 else t.contiguous()
+
+
 def _attention_args(what, q, k, v, kv_lens, kv_mask, scale, more=()):
     """Checked tensors of a cross attention call: (q, k, v, pointers of kv_lens and kv_mask, what holds them, scale, sizes, type code)."""
     code = _operands(what, q, (k, v, *more), (kv_lens, kv_mask))
@@ -1883,13 +1889,7 @@ def _attention_args(what, q, k, v, kv_lens, kv_mask, scale, more=()):
         scale = D ** -0.5
     elif not 0.0 < scale < float("inf"):
         raise _lib.DfsfmError(f"{what}: the scale is positive")
-    if q.stride(3) != 1:
-        q = q.contiguous()
-    if k.stride(3) != 1:
-        k = k.contiguous()
-    if v.stride(3) != 1:
-        v = v.contiguous()
-    return q, k, v, lens, mask, (kv_lens, kv_mask), scale, (N, L, S, H, Hkv, D), code
+    return _heads(q), _heads(k), _heads(v), lens, mask, (kv_lens, kv_mask), scale, (N, L, S, H, Hkv, D), code
 
 
 def _heads_ptr(t):
@@ -1929,11 +1929,7 @@ def cross_attention_backward(dout, q, k, v, out, lse, kv_lens=None, kv_mask=None
         raise _lib.DfsfmError("cross_attention_backward: dout and out have q's shape and type")
     if lse.shape != (N, H, L) or lse.dtype != torch.float32 or lse.get_device() != q.get_device():
         raise _lib.DfsfmError("cross_attention_backward: lse is what cross_attention returned, fp32 [N, H, L]")
-    if dout.stride(3) != 1:
-        dout = dout.contiguous()
-    if out.stride(3) != 1:
-        out = out.contiguous()
-    lse = lse.contiguous()
+    dout, out, lse = _heads(dout), _heads(out), lse.contiguous()
     dq = torch.empty_like(q, memory_format=torch.contiguous_format)
     dk, dv = torch.empty_like(k, memory_format=torch.contiguous_format), torch.empty_like(v, memory_format=torch.contiguous_format)
     lib = _lib.lib()
