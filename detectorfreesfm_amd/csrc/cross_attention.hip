@@ -62,48 +62,61 @@ __device__ __forceinline__ Frag<T> zero_frag() {
     return f;
 }
 
-// 8 consecutive channels from global memory (any alignment)
+// 8 consecutive channels from global memory
 template <typename T>
 __device__ __forceinline__ Frag<T> load8(const T* p) {
-    typedef typename dfsfm::Vec<T, 8>::type vec;
-    return *reinterpret_cast<const vec*>(p);
+    typedef Frag<T> at16 __attribute__((aligned(16)));
+    return *reinterpret_cast<const at16*>(p);
 }
 
-// Row pitches of a tile in LDS, in elements.  Rows read as A operands (16 bytes a lane, a row a lane): pitch = DP + 16 bytes.  Rows read
-// transposed (four rows x 32 bytes by 16 lanes): DP + 32 bytes.  Both spread the lanes of a cycle over all banks.
+// How a tile of DP channels a row lies in LDS, and where this lane reads it.  Both ways of reading have to spread over all 64 banks: as A
+// operands (16 bytes a lane, a row a lane) and transposed (16 lanes read four rows x 32 bytes).  Rows have no padding (the tile is written
+// by LDS-DMA, 1 KB of consecutive LDS an instruction); their 16-byte chunks are permuted by the row number: chunk c of row r lies at c ^
+// order(r), where order() differs by at least four chunks between neighbouring rows that share banks (the transposed read) and takes every
+// value over 16 rows (the other).  A lane's row is the same modulo 16 in every read, so the permutation is one exclusive or with a
+// constant.  Padded rows (272 or 288 bytes) cost the dk / dv kernel 35 % of its LDS cycles in conflicts; this order has none.
 template <typename T, int DP>
-constexpr int PITCH = DP + 16 / sizeof(T);
-template <typename T, int DP>
-constexpr int PITCH_T = DP + 32 / sizeof(T);
-
-// A operand: rows row .. row + 31 of a tile, inner index = channels col .. col + 15.
-template <typename T>
-__device__ __forceinline__ Frag<T> read_rows(const T* tile, int pitch, int row, int col, int lane) {
-    typedef Frag<T> at16 __attribute__((aligned(16)));                    // pitches are multiples of 16 bytes, not of 32
-    return *reinterpret_cast<const at16*>(tile + (row + (lane & 31)) * pitch + col + 8 * (lane >> 5));
-}
-
-// A operand of the transposed tile: rows = channels col .. col + 31, inner index = tile rows in the order of an accumulator's registers:
-// slot j of half h is row + (j & 3) + 8 (j >> 2) + 4 h.
-template <typename T>
-__device__ __forceinline__ Frag<T> read_cols(const T* tile, int pitch, int row, int col, int lane) {
-    if constexpr (sizeof(T) == 2) {
-        // 16 lanes read a 4 x 16 block, 8 bytes each along its rows; the transposed read hands lane i the block's column i
-        const int i = lane & 15;
-        const T* p = tile + (row + 4 * (lane >> 5) + (i >> 2)) * pitch + col + (lane & 16) + 4 * (i & 3);
-        typedef __attribute__((address_space(3))) s16x4* lds_ptr;
-        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p);
-        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 8 * pitch));
-        const auto v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-        return __builtin_bit_cast(Frag<T>, v);
-    } else {
-        Frag<T> f;
-        const T* p = tile + (row + 4 * (lane >> 5)) * pitch + col + (lane & 31);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = p[((j & 3) + 8 * (j >> 2)) * pitch];
-        return f;
+struct Lds {
+    static constexpr bool HALF = sizeof(T) == 2;
+    static constexpr int CH = DP * sizeof(T) / 16, E = 16 / sizeof(T);    // chunks a row, elements a chunk
+    static constexpr int TILE = KT * DP;                                  // elements of 64 rows
+    int rows, cols;                                                       // this lane's offsets
+    static __host__ __device__ constexpr int order(int r) {
+        return CH >= 16 ? (r & 3) << 2 | (r >> 2 & 3) : CH == 8 ? (r >> 1 & 1) << 2 | (r >> 2 & 3) : r >> 2 & 3;
     }
-}
+    __device__ __forceinline__ explicit Lds(int lane) {
+        const int i = lane & 15, half = lane >> 5, r = 4 * half + (i >> 2);
+        rows = (lane & 31) * DP + ((HALF ? half : 2 * half) ^ order(lane & 31)) * E;
+        cols = HALF ? r * DP + (((lane & 16) / 8 + (i >> 1 & 1)) ^ order(r)) * E + 4 * (i & 1) : 4 * half * DP + ((lane & 31) ^ order(4 * half) * E);
+    }
+    // A operand: rows row .. row + 31 (row: a multiple of 32), inner index = channels col .. col + 15
+    __device__ __forceinline__ Frag<T> read_rows(const T* tile, int row, int col) const {
+        const T* p = tile + row * DP;
+        if constexpr (HALF) {
+            return *reinterpret_cast<const Frag<T>*>(p + (rows ^ col));
+        } else {
+            const f32x4 u = *reinterpret_cast<const f32x4*>(p + (rows ^ col)), v = *reinterpret_cast<const f32x4*>(p + (rows ^ col ^ E));
+            return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+    // A operand of the transposed tile: rows = channels col .. col + 31, inner index = tile rows row .. row + 15 in the order of an
+    // accumulator's registers: slot j of half h is row + (j & 3) + 8 (j >> 2) + 4 h
+    __device__ __forceinline__ Frag<T> read_cols(const T* tile, int row, int col) const {
+        const T* p = tile + row * DP;
+        if constexpr (HALF) {
+            // 16 lanes read a 4 x 16 block, 8 bytes each along its rows; the transposed read hands lane i the block's column i
+            typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + (cols ^ col)));
+            const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 8 * DP + (cols ^ col ^ order(8) * E)));
+            return __builtin_bit_cast(Frag<T>, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            Frag<T> f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = p[((j & 3) + 8 * (j >> 2)) * DP + (cols ^ col ^ order((j & 3) + 8 * (j >> 2)) * E)];
+            return f;
+        }
+    }
+};
 
 // Registers 8 t .. 8 t + 7 of a score tile as the other operand (round to nearest even).
 template <typename T>
@@ -154,49 +167,66 @@ struct Job {
 
 __device__ __forceinline__ int valid_len(const Attn& a, int n) { return a.lens ? min(max(a.lens[n], 0), a.S) : a.S; }
 
-// A tile of 64 rows x DP channels on its way from memory through the registers of 256 threads into LDS.  A thread's 32-bit byte offsets
-// within a tile are the same for every whole tile: the address costs one scalar base a tile and no vector arithmetic.
-template <typename T, int DP>
-struct Stage {
-    static constexpr int VPR = DP / 8, PER = KT * VPR / 256;
-    Frag<T> r[PER];
-    unsigned off[PER];
-    unsigned stride;                       // bytes a row
-    int D;
-    __device__ __forceinline__ Stage(int64_t stride_, int D_) : stride((unsigned)(stride_ * sizeof(T))), D(D_) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) off[i] = offset(i, KT - 1);
+// A tile of ROWS rows x DP channels on its way from memory into LDS, by LDS-DMA: no register holds it and no vector instruction moves it.
+// Every thread fetches 16 bytes an instruction; the chunk order of Lds is applied to the source address.  Rows behind the last and channels
+// behind D lie outside the buffer descriptor and arrive as zeros.
+template <typename T, int DP, int ROWS, int THREADS>
+struct Dma {
+    typedef Lds<T, DP> L;
+    static constexpr int CH = L::CH, PER = ROWS * CH / THREADS, RPI = THREADS / CH;   // instructions a tile, rows an instruction
+    unsigned off, step, row_bytes, stride;
+    __device__ __forceinline__ Dma(int64_t stride_, int D) : stride((unsigned)(stride_ * sizeof(T))) {
+        row_bytes = D * (unsigned)sizeof(T);
+        off = threadIdx.x / CH * stride;
+        step = RPI * stride;
     }
-    __device__ __forceinline__ unsigned offset(int i, int last) const {
-        const int e = threadIdx.x + 256 * i;
-        return min(e / VPR, last) * stride + e % VPR * 8 * (unsigned)sizeof(T);
-    }
-    // rows base .. base + rows - 1, the last one again behind them
-    __device__ __forceinline__ void load(const T* base, int rows) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const unsigned o = rows >= KT ? off[i] : offset(i, rows - 1);
-            const T* p = reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + o);
-            r[i] = (threadIdx.x + 256 * i) % VPR * 8 < D ? load8<T>(p) : zero_frag<T>();
-        }
-    }
-    // rows whose bit in `keep` is 0 become zeros
-    __device__ __forceinline__ void store(T* tile, int pitch, unsigned long long keep) const {
-        typedef Frag<T> at16 __attribute__((aligned(16)));
+    // rows base .. base + rows - 1 (rows > 0); base, rows and tile are the same in every lane
+    __device__ __forceinline__ void issue(const T* base, int rows, T* tile) const {
+        typedef int i32x4 __attribute__((ext_vector_type(4)));
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const uint64_t at = reinterpret_cast<uint64_t>(base);
+        const i32x4 rsrc = {__builtin_amdgcn_readfirstlane((int)at), __builtin_amdgcn_readfirstlane((int)(at >> 32) & 0xffff),
+                            __builtin_amdgcn_readfirstlane((int)((unsigned)(min(rows, ROWS) - 1) * stride + row_bytes)), 0x00020000};
+        const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) void*)tile) + wave * 1024;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int e = threadIdx.x + 256 * i, row = e / VPR, c = e % VPR * 8;
-            *reinterpret_cast<at16*>(tile + row * pitch + c) = ~keep == 0 || keep >> row & 1 ? r[i] : zero_frag<T>();
+            const unsigned c = (threadIdx.x % CH ^ L::order(threadIdx.x / CH) ^ L::order(RPI * i & 15)) * 16;
+            // channels behind D: an offset no descriptor reaches (strides are below 2^23 elements)
+            const unsigned o = c < row_bytes ? off + step * i + c : 0xff000000u;
+            // As assembly (it writes no register) because the compiler lets every LDS read wait for its own form of this load.  The waits:
+            // five states from a lane read's scalar to a memory instruction that uses it, one from m0.
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to + i * THREADS * 16), "v"(o), "s"(rsrc) : "memory", "m0");
         }
     }
 };
 
+__device__ __forceinline__ void dma_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Zeros over the rows whose bit in `keep` is 0, by 256 threads.
+template <typename T, int DP>
+__device__ __forceinline__ void zero_rows(T* tile, unsigned long long keep) {
+    constexpr int CH = Lds<T, DP>::CH;
+    unsigned e = threadIdx.x;
+    asm volatile("" : "+v"(e));            // keeps this branch's addresses out of the loop's registers
+#pragma unroll
+    for (int i = 0; i < KT * CH / 256; ++i, e += 256)
+        if (!(keep >> (e / CH) & 1)) *reinterpret_cast<f32x4*>(tile + e * Lds<T, DP>::E) = f32x4{0.f, 0.f, 0.f, 0.f};
+}
+
+// The mask byte of key s0 + lane, one tile ahead of its use; 1 without a mask.
+__device__ __forceinline__ unsigned key_mask(const Attn& a, int n, int s0) {
+    return a.mask ? a.mask[(int64_t)n * a.S + min(s0 + (int)(threadIdx.x & 63), a.S - 1)] : 1u;
+}
+
 // Bits of the keys s0 .. s0 + 63 that are there; the same in every wave.
-__device__ __forceinline__ unsigned long long key_bits(const Attn& a, int n, int s0, int end) {
-    const int s = s0 + (threadIdx.x & 63);
-    bool ok = s < end;
-    if (a.mask) ok = ok && a.mask[(int64_t)n * a.S + min(s, a.S - 1)] != 0;
-    return __ballot(ok);
+__device__ __forceinline__ unsigned long long key_bits(unsigned mask, int s0, int end) {
+    return __ballot(s0 + (int)(threadIdx.x & 63) < end && mask != 0);
+}
+
+// Scores of keys that are not there become -inf, whatever they were: bits of 32 keys, this lane's half shifted to bit 0.
+__device__ __forceinline__ void drop_keys(f32x16& st, unsigned bits) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) st[j] = bits >> mfma32_row(j, 0) & 1 ? st[j] : NEG;
 }
 
 __device__ __forceinline__ f32x16 splat16(float x) {
@@ -284,13 +314,13 @@ struct ColumnScale {
 // 4 waves x 32 rows a workgroup; tiles of 64 keys, two in LDS.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_forward_kernel(const Attn a) {
-    constexpr int KP = PITCH<T, DP>, VP = PITCH_T<T, DP>, DB = DP / 32, KS = DP / 16;
+    constexpr int DB = DP / 32, KS = DP / 16, TILE = Lds<T, DP>::TILE;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* ks = reinterpret_cast<T*>(smem);
-    T* vs = ks + 2 * KT * KP;
-    float* bias = reinterpret_cast<float*>(vs + 2 * KT * VP);            // [2][64]
+    T* vs = ks + 2 * TILE;
     const Job job(a);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Lds<T, DP> lds(lane);
     const int R = a.L * a.G, r = job.tile * 128 + wave * 32 + (lane & 31);
     const int l = r / a.G, h = job.hk * a.G + r % a.G;
     const int len = valid_len(a, job.n);
@@ -306,35 +336,43 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_forward_kernel(const
     }
     const T* kb = static_cast<const T*>(a.k.p) + job.n * a.k.n + job.hk * a.k.h;
     const T* vb = static_cast<const T*>(a.v.p) + job.n * a.v.n + job.hk * a.v.h;
-    Stage<T, DP> sk(a.k.l, a.D), sv(a.v.l, a.D);
-    auto fetch = [&](int s0) {
-        sk.load(kb + s0 * a.k.l, end - s0);
-        sv.load(vb + s0 * a.v.l, end - s0);
+    const Dma<T, DP, KT, 256> dk(a.k.l, a.D), dv(a.v.l, a.D);
+    unsigned mask = 0;
+    auto fetch = [&](int s0, int buf) {
+        dk.issue(kb + s0 * a.k.l, end - s0, ks + buf * TILE);
+        dv.issue(vb + s0 * a.v.l, end - s0, vs + buf * TILE);
+        mask = key_mask(a, job.n, s0);
     };
     f32x16 acc[DB];
 #pragma unroll
     for (int b = 0; b < DB; ++b) acc[b] = splat16(0.f);
     float m = NEG, sum = 0.f;               // maximum of scale * log2(e) * q k, sum of this lane's half of the keys
     const float c = a.scale * LOG2E;
-    if (beg < end) fetch(beg);
+    if (beg < end) fetch(beg, 0);
     int buf = 0;
     for (int s0 = beg; s0 < end; s0 += KT, buf ^= 1) {
-        const unsigned long long bits = key_bits(a, job.n, s0, end);
-        T* kt = ks + buf * KT * KP;
-        T* vt = vs + buf * KT * VP;
-        float* bt = bias + buf * KT;
-        sk.store(kt, KP, bits);
-        sv.store(vt, VP, bits);
-        if (threadIdx.x < KT) bt[threadIdx.x] = bits >> threadIdx.x & 1 ? 0.f : NEG;
-        __syncthreads();                    // the other buffer's readers passed the barrier before this tile's writers came here
-        if (s0 + KT < end) fetch(s0 + KT);
+        const T* kt = ks + buf * TILE;
+        T* vt = vs + buf * TILE;
+        dma_landed();
+        const unsigned long long bits = key_bits(mask, s0, end);
+        __syncthreads();                    // all of the tile is there, and the other buffer's readers are done
+        if (a.mask && ~bits && bits) {      // a weight of 0 does not undo a NaN in v
+            zero_rows<T, DP>(vt, bits);
+            __syncthreads();
+        }
+        if (s0 + KT < end) fetch(s0 + KT, buf ^ 1);
         if (bits == 0) continue;
         f32x16 st[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            st[b] = ~bits ? rows16(bt + 32 * b, lane) : splat16(0.f);
+            st[b] = splat16(0.f);
 #pragma unroll
-            for (int s = 0; s < KS; ++s) st[b] = Mma<T>::run(read_rows(kt, KP, 32 * b, 16 * s, lane), qf[s], st[b]);
+            for (int s = 0; s < KS; ++s) st[b] = Mma<T>::run(lds.read_rows(kt, 32 * b, 16 * s), qf[s], st[b]);
+        }
+        if (~bits) {
+            const unsigned long long mine = bits >> 4 * (lane >> 5);
+            drop_keys(st[0], (unsigned)mine);
+            drop_keys(st[1], (unsigned)(mine >> 32));
         }
         float t = NEG;
 #pragma unroll
@@ -342,8 +380,9 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_forward_kernel(const
 #pragma unroll
             for (int j = 0; j < 16; ++j) t = fmaxf(t, st[b][j]);
         t = fmaxf(t, dfsfm::from_xor32(t, lane)) * c;
-        if (__ballot(t > m)) {
-            const float mn = fmaxf(m, t), f = m == NEG ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+        // the reference follows the maximum once it is 8 behind: weights up to 2^8 lose nothing, and most tiles rescale nothing
+        if (__ballot(t > m + 8.f)) {
+            const float mn = t > m + 8.f ? t : m, f = m == NEG ? 0.f : __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             sum *= f;
 #pragma unroll
@@ -363,7 +402,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_forward_kernel(const
             for (int u = 0; u < 2; ++u) {
                 const Frag<T> p = pack8<T>(st[b], u);
 #pragma unroll
-                for (int d = 0; d < DB; ++d) acc[d] = Mma<T>::run(read_cols(vt, VP, 32 * b + 16 * u, 32 * d, lane), p, acc[d]);
+                for (int d = 0; d < DB; ++d) acc[d] = Mma<T>::run(lds.read_cols(vt, 32 * b + 16 * u, 32 * d), p, acc[d]);
             }
         }
     }
@@ -442,13 +481,13 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(const Attn a) {
 // costs).  Two of three products are then made twice, over two tiles at most; a pass over dout and out is saved.
 template <typename T, int DP, bool SHORT>
 __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn a) {
-    constexpr int KP = PITCH_T<T, DP>, VP = PITCH<T, DP>, DB = DP / 32, KS = DP / 16;
+    constexpr int DB = DP / 32, KS = DP / 16, TILE = Lds<T, DP>::TILE;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* ks = reinterpret_cast<T*>(smem);
-    T* vs = ks + 2 * KT * KP;
-    float* bias = reinterpret_cast<float*>(vs + 2 * KT * VP);
+    T* vs = ks + 2 * TILE;
     const Job job(a);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Lds<T, DP> lds(lane);
     const int R = a.L * a.G, r = job.tile * 128 + wave * 32 + (lane & 31);
     const int l = r / a.G, h = job.hk * a.G + r % a.G;
     const int len = valid_len(a, job.n);
@@ -470,67 +509,76 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
     float delta = !SHORT && r < R ? a.delta[at] : 0.f;
     const T* kb = static_cast<const T*>(a.k.p) + job.n * a.k.n + job.hk * a.k.h;
     const T* vb = static_cast<const T*>(a.v.p) + job.n * a.v.n + job.hk * a.v.h;
-    Stage<T, DP> sk(a.k.l, a.D), sv(a.v.l, a.D);
-    auto fetch = [&](int s0) {
-        sk.load(kb + s0 * a.k.l, end - s0);
-        sv.load(vb + s0 * a.v.l, end - s0);
+    const Dma<T, DP, KT, 256> dk(a.k.l, a.D), dv(a.v.l, a.D);
+    unsigned mask = 0;
+    auto fetch = [&](int s0, int buf) {
+        dk.issue(kb + s0 * a.k.l, end - s0, ks + buf * TILE);
+        dv.issue(vb + s0 * a.v.l, end - s0, vs + buf * TILE);
+        mask = key_mask(a, job.n, s0);
     };
-    auto stage = [&](int s0, int buf) {
-        const unsigned long long bits = key_bits(a, job.n, s0, end);
-        sk.store(ks + buf * KT * KP, KP, bits);
-        sv.store(vs + buf * KT * VP, VP, bits);
-        if (threadIdx.x < KT) bias[buf * KT + threadIdx.x] = bits >> threadIdx.x & 1 ? 0.f : NEG;
-        return bits;
+    // keys that the mask drops: p is 0, which does not undo a NaN in dp or k
+    auto clear = [&](int buf, unsigned long long bits) {
+        if (a.mask && ~bits && bits) {
+            zero_rows<T, DP>(ks + buf * TILE, bits);
+            zero_rows<T, DP>(vs + buf * TILE, bits);
+            __syncthreads();
+        }
     };
     f32x16 acc[DB];
 #pragma unroll
     for (int b = 0; b < DB; ++b) acc[b] = splat16(0.f);
     ColumnScale<T, DB> cs;
     // p dp of 32 keys, dp less delta
-    auto products = [&](int buf, int b, bool whole, f32x16& ds) {
-        const T* kt = ks + buf * KT * KP;
-        const T* vt = vs + buf * KT * VP;
-        f32x16 st = whole ? splat16(0.f) : rows16(bias + buf * KT + 32 * b, lane);
+    auto products = [&](int buf, int b, unsigned long long bits, f32x16& ds) {
+        const T* kt = ks + buf * TILE;
+        const T* vt = vs + buf * TILE;
+        f32x16 st = splat16(0.f);
         ds = splat16(-delta);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            st = Mma<T>::run(read_rows(kt, KP, 32 * b, 16 * s, lane), qf[s], st);
-            ds = Mma<T>::run(read_rows(vt, VP, 32 * b, 16 * s, lane), of[s], ds);
+            st = Mma<T>::run(lds.read_rows(kt, 32 * b, 16 * s), qf[s], st);
+            ds = Mma<T>::run(lds.read_rows(vt, 32 * b, 16 * s), of[s], ds);
         }
+        if (~bits) drop_keys(st, (unsigned)(bits >> 32 * b >> 4 * (lane >> 5)));
 #pragma unroll
         for (int j = 0; j < 16; ++j) ds[j] *= __builtin_amdgcn_exp2f(fmaf(st[j], c, -lse2));
     };
-    auto accumulate = [&](int buf, bool whole) {
+    auto accumulate = [&](int buf, unsigned long long bits) {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             f32x16 ds[1];
-            products(buf, b, whole, ds[0]);
+            products(buf, b, bits, ds[0]);
             cs.apply(ds, acc);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const Frag<T> p = pack8<T>(ds[0], u);
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
-                    acc[d] = Mma<T>::run(read_cols(ks + buf * KT * KP, KP, 32 * b + 16 * u, 32 * d, lane), p, acc[d]);
+                    acc[d] = Mma<T>::run(lds.read_cols(ks + buf * TILE, 32 * b + 16 * u, 32 * d), p, acc[d]);
             }
         }
     };
-    if (beg < end) fetch(beg);
     if constexpr (SHORT) {
         unsigned long long bits[2] = {0, 0};
+        unsigned masks[2] = {0, 0};
 #pragma unroll
         for (int t = 0; t < 2; ++t)
             if (t * KT < end) {
-                bits[t] = stage(t * KT, t);
-                if (t == 0 && KT < end) fetch(KT);
+                fetch(t * KT, t);
+                masks[t] = mask;
             }
+        dma_landed();
+#pragma unroll
+        for (int t = 0; t < 2; ++t) bits[t] = key_bits(masks[t], t * KT, end);
         __syncthreads();
+        clear(0, bits[0]);
+        clear(1, bits[1]);
         float sum = 0.f;
         for (int t = 0; t * KT < end; ++t)
             if (bits[t]) {
                 for (int b = 0; b < 2; ++b) {
                     f32x16 ds;
-                    products(t, b, ~bits[t] == 0, ds);
+                    products(t, b, bits[t], ds);
 #pragma unroll
                     for (int j = 0; j < 16; ++j) sum += ds[j];
                 }
@@ -538,14 +586,17 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
         delta = dfsfm::add_xor32(sum);
         if (r < R && lane < 32) a.delta[at] = delta;
         for (int t = 0; t * KT < end; ++t)
-            if (bits[t]) accumulate(t, ~bits[t] == 0);
+            if (bits[t]) accumulate(t, bits[t]);
     } else {
+        if (beg < end) fetch(beg, 0);
         int buf = 0;
         for (int s0 = beg; s0 < end; s0 += KT, buf ^= 1) {
-            const unsigned long long bits = stage(s0, buf);
+            dma_landed();
+            const unsigned long long bits = key_bits(mask, s0, end);
             __syncthreads();
-            if (s0 + KT < end) fetch(s0 + KT);
-            if (bits) accumulate(buf, ~bits == 0);
+            clear(buf, bits);
+            if (s0 + KT < end) fetch(s0 + KT, buf ^ 1);
+            if (bits) accumulate(buf, bits);
         }
     }
     if (r >= R) return;
@@ -560,15 +611,16 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
 // dk and dv: 4 waves x 32 keys a workgroup, tiles of 64 rows of q and dout, both read both ways.
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void attn_dkdv_kernel(const Attn a) {
-    constexpr int P = PITCH_T<T, DP>, DB = DP / 32, KS = DP / 16;
+    constexpr int DB = DP / 32, KS = DP / 16, TILE = Lds<T, DP>::TILE;
     // p of fp16 tensors times 2^14: a power of two that keeps weights down to 2^-28 exact and 1 in range
     constexpr float SHIFT = __is_same(T, f16) ? 14.f : 0.f, UNSHIFT = __is_same(T, f16) ? 1.f / 16384.f : 1.f;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* qs = reinterpret_cast<T*>(smem);
-    T* os = qs + 2 * KT * P;
-    float* rowv = reinterpret_cast<float*>(os + 2 * KT * P);              // [2][2][64]: -lse / scale, -delta
+    T* os = qs + 2 * TILE;
+    float* rowv = reinterpret_cast<float*>(os + 2 * TILE);                // [2][2][64]: -lse / scale, -delta
     const Job job(a);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hkv = a.H / a.G;
+    const Lds<T, DP> lds(lane);
     const int s = job.tile * 128 + wave * 32 + (lane & 31);
     const int len = valid_len(a, job.n);
     bool there = s < len;
@@ -589,20 +641,18 @@ __global__ __launch_bounds__(256) void attn_dkdv_kernel(const Attn a) {
     const T* qb = static_cast<const T*>(a.q.p) + job.n * a.q.n + job.hk * a.G * a.q.h;
     const T* ob = static_cast<const T*>(a.dout.p) + job.n * a.dout.n + job.hk * a.G * a.dout.h;
     const int64_t vec = ((int64_t)job.n * a.H + job.hk * a.G) * a.L;
-    Stage<T, DP> sq(a.q.l, a.D), so(a.dout.l, a.D);
-    float rv = 0.f;                         // threads 0..63: -lse / scale of a row, 64..127: -delta
+    const Dma<T, DP, KT, 256> dq(a.q.l, a.D), dd(a.dout.l, a.D);
+    float rv = 0.f;                         // threads 0..63: lse of a row, 64..127: delta
+    const float inv_scale = 1.f / a.scale;
     int rows = 0;                           // rows of the tile in flight
-    auto fetch = [&](int it) {
+    auto fetch = [&](int it, int buf) {
         const int g = it / lt, l0 = (it - g * lt) * KT;
         rows = a.L - l0;
-        sq.load(qb + g * a.q.h + l0 * a.q.l, rows);
-        so.load(ob + g * a.dout.h + l0 * a.dout.l, rows);
+        dq.issue(qb + g * a.q.h + l0 * a.q.l, rows, qs + buf * TILE);
+        dd.issue(ob + g * a.dout.h + l0 * a.dout.l, rows, os + buf * TILE);
         if (threadIdx.x < 128) {
             const int row = threadIdx.x & 63;
-            const int64_t at = vec + (int64_t)g * a.L + l0 + min(row, rows - 1);
-            const float t = threadIdx.x < 64 ? a.lse[at] : a.delta[at];
-            // a row without keys, or behind the last: a score of -inf, p = 0
-            rv = threadIdx.x < 64 ? (row < rows && t != NEG ? -t / a.scale : NEG) : (row < rows ? -t : 0.f);
+            rv = (threadIdx.x < 64 ? a.lse : a.delta)[vec + (int64_t)g * a.L + l0 + min(row, rows - 1)];
         }
     };
     f32x16 dk[DB], dv[DB];
@@ -611,18 +661,20 @@ __global__ __launch_bounds__(256) void attn_dkdv_kernel(const Attn a) {
     ColumnScale<T, DB> cs;
     const float c = a.scale * LOG2E;
     const bool any = __syncthreads_or(there);
-    if (any && beg < end) fetch(beg);
+    if (any && beg < end) fetch(beg, 0);
     int buf = 0;
     for (int it = beg; any && it < end; ++it, buf ^= 1) {
-        T* qt = qs + buf * KT * P;
-        T* ot = os + buf * KT * P;
+        T* qt = qs + buf * TILE;
+        T* ot = os + buf * TILE;
         float* vt = rowv + buf * 128;
-        const unsigned long long keep = rows >= KT ? ~0ull : (1ull << rows) - 1;
-        sq.store(qt, P, keep);
-        so.store(ot, P, keep);
-        if (threadIdx.x < 128) vt[threadIdx.x] = rv;
+        dma_landed();
+        // -lse / scale and -delta start the sums; a row without keys, or behind the last, gets a score of -inf: p = 0
+        if (threadIdx.x < 128) {
+            const bool in = (int)(threadIdx.x & 63) < rows;
+            vt[threadIdx.x] = threadIdx.x < 64 ? (in && rv != NEG ? -rv * inv_scale : NEG) : (in ? -rv : 0.f);
+        }
         __syncthreads();
-        if (it + 1 < end) fetch(it + 1);
+        if (it + 1 < end) fetch(it + 1, buf ^ 1);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             f32x16 st = rows16(vt + 32 * b, lane);
@@ -630,8 +682,8 @@ __global__ __launch_bounds__(256) void attn_dkdv_kernel(const Attn a) {
             ds[0] = rows16(vt + 64 + 32 * b, lane);
 #pragma unroll
             for (int x = 0; x < KS; ++x) {
-                st = Mma<T>::run(read_rows(qt, P, 32 * b, 16 * x, lane), kf[x], st);
-                ds[0] = Mma<T>::run(read_rows(ot, P, 32 * b, 16 * x, lane), vf[x], ds[0]);
+                st = Mma<T>::run(lds.read_rows(qt, 32 * b, 16 * x), kf[x], st);
+                ds[0] = Mma<T>::run(lds.read_rows(ot, 32 * b, 16 * x), vf[x], ds[0]);
             }
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
@@ -644,8 +696,8 @@ __global__ __launch_bounds__(256) void attn_dkdv_kernel(const Attn a) {
                 const Frag<T> p = pack8<T>(st, u), g = pack8<T>(ds[0], u);
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
-                    dv[d] = Mma<T>::run(read_cols(ot, P, 32 * b + 16 * u, 32 * d, lane), p, dv[d]);
-                    dk[d] = Mma<T>::run(read_cols(qt, P, 32 * b + 16 * u, 32 * d, lane), g, dk[d]);
+                    dv[d] = Mma<T>::run(lds.read_cols(ot, 32 * b + 16 * u, 32 * d), p, dv[d]);
+                    dk[d] = Mma<T>::run(lds.read_cols(qt, 32 * b + 16 * u, 32 * d), g, dk[d]);
                 }
             }
         }
@@ -666,6 +718,169 @@ __global__ __launch_bounds__(256) void attn_dkdv_kernel(const Attn a) {
     }
 }
 
+// dk and dv for D = 128 in 16 bits: one wave's K, V, dk and dv need 192 registers before the first score, which leaves one wave a SIMD and
+// nothing to run beside its exponentials.  Here two waves share 32 keys: waves 0 .. 3 make p and dv, waves 4 .. 7 dp, ds and dk, half of the
+// products each and half of the registers.  p goes through LDS in 32 bits, lane to lane in accumulator order, one tile behind: while a first
+// wave is at tile i, its partner is at tile i - 1.  Every operand is on its way from LDS a product ahead: a tile's score operands while the
+// tile before is accumulated, the transposed ones before the exponentials.  Tiles are 32 rows, four in LDS: i - 1 .. i + 1 being read, i + 2
+// being written.
+template <typename T>
+__global__ __launch_bounds__(512, 2) void attn_dkdv_pair_kernel(const Attn a) {
+    constexpr int DP = 128, DB = DP / 32, KS = DP / 16, QT = 32, TILE = Lds<T, DP>::TILE / 2;
+    constexpr float SHIFT = __is_same(T, f16) ? 14.f : 0.f, UNSHIFT = __is_same(T, f16) ? 1.f / 16384.f : 1.f;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    T* qs = reinterpret_cast<T*>(smem);                                   // [4][32][DP]
+    T* os = qs + 4 * TILE;
+    float* ps = reinterpret_cast<float*>(os + 4 * TILE);                  // [2][4 pairs][4][64 lanes] x 4
+    float* rowv = ps + 2 * 4 * 1024;                                      // [4][2][32]: -lse / scale, -delta
+    const Job job(a);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pair = wave & 3, hkv = a.H / a.G;
+    const bool first = wave < 4;
+    const Lds<T, DP> lds(lane);
+    const int s = job.tile * 128 + pair * 32 + (lane & 31);
+    const int len = valid_len(a, job.n);
+    bool there = s < len;
+    if (a.mask) there = there && a.mask[(int64_t)job.n * a.S + min(s, a.S - 1)] != 0;
+    const int lt = (a.L + QT - 1) / QT, per = (lt * a.G + a.splits - 1) / a.splits;
+    const int beg = min(lt * a.G, job.split * per), end = min(lt * a.G, beg + per);
+
+    Frag<T> kv[KS];                         // K of a first wave, V of a second
+    const Tensor& own = first ? a.k : a.v;
+    const T* kp = static_cast<const T*>(own.p) + job.n * own.n + (int64_t)min(s, a.S - 1) * own.l + job.hk * own.h;
+#pragma unroll
+    for (int x = 0; x < KS; ++x) {
+        const int c = 16 * x + 8 * (lane >> 5);
+        kv[x] = there && c < a.D ? load8<T>(kp + c) : zero_frag<T>();
+    }
+    const T* qb = static_cast<const T*>(a.q.p) + job.n * a.q.n + job.hk * a.G * a.q.h;
+    const T* ob = static_cast<const T*>(a.dout.p) + job.n * a.dout.n + job.hk * a.G * a.dout.h;
+    const int64_t vec = ((int64_t)job.n * a.H + job.hk * a.G) * a.L;
+    const Dma<T, DP, QT, 512> dq(a.q.l, a.D), dd(a.dout.l, a.D);
+    const float inv_scale = 1.f / a.scale;
+    float rv = 0.f;                         // threads 0..31: lse of a row, 32..63: delta
+    int rows = 0;                           // rows of the tile in flight
+    auto fetch = [&](int i) {               // tile beg + i
+        const int it = beg + i, g = it / lt, l0 = (it - g * lt) * QT;
+        rows = a.L - l0;
+        dq.issue(qb + g * a.q.h + l0 * a.q.l, rows, qs + (i & 3) * TILE);
+        dd.issue(ob + g * a.dout.h + l0 * a.dout.l, rows, os + (i & 3) * TILE);
+        if (threadIdx.x < 64) rv = (threadIdx.x < 32 ? a.lse : a.delta)[vec + (int64_t)g * a.L + l0 + min((int)threadIdx.x & 31, rows - 1)];
+    };
+    auto put = [&](int i) {                 // its row values, once they are here
+        if (threadIdx.x < 64) {
+            const bool in = (int)(threadIdx.x & 31) < rows;
+            rowv[(i & 3) * 64 + threadIdx.x] = threadIdx.x < 32 ? (in && rv != NEG ? -rv * inv_scale : NEG) : (in ? -rv : 0.f);
+        }
+    };
+    f32x16 acc[DB];                         // dv of a first wave, dk of a second
+#pragma unroll
+    for (int b = 0; b < DB; ++b) acc[b] = splat16(0.f);
+    ColumnScale<T, DB> cs;
+    const float c = a.scale * LOG2E;
+    Frag<T> f[KS];                          // score operands of the tile at hand
+    f32x16 start;
+    auto ahead = [&](const T* tile, const float* from) {
+#pragma unroll
+        for (int x = 0; x < KS; ++x) f[x] = lds.read_rows(tile, 0, 16 * x);
+        start = rows16(from, lane);
+    };
+    auto scores = [&]() {
+        f32x16 st = start;
+#pragma unroll
+        for (int x = 0; x < KS; ++x) st = Mma<T>::run(f[x], kv[x], st);
+        return st;
+    };
+    const bool any = __syncthreads_or(there) && beg < end;
+    if (any) {
+        const int n = end - beg;
+        fetch(0);
+        dma_landed();
+        put(0);
+        if (n > 1) fetch(1);
+        // Past the barrier tile i + 1 is in LDS, and tile i + 2 leaves memory for the place of tile i - 2, whose readers are done.
+        auto turn = [&](int i) {
+            dma_landed();
+            if (i + 1 < n) put(i + 1);
+            __syncthreads();
+            if (i + 2 < n) fetch(i + 2);
+        };
+        // both halves pass n + 1 barriers
+        if (first) {
+            for (int i = 0; i < n; ++i) {
+                turn(i);
+                if (i == 0) ahead(qs, rowv);
+                f32x16 st = scores();
+                Frag<T> w[2][DB];
+                const T* ot = os + (i & 3) * TILE;
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) w[u][d] = lds.read_cols(ot, 16 * u, 32 * d);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) st[j] = __builtin_amdgcn_exp2f(fmaf(st[j], c, SHIFT));
+                float* pt = ps + ((i & 1) * 4 + pair) * 1024 + 4 * lane;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) *reinterpret_cast<f32x4*>(pt + 256 * g) = f32x4{st[4 * g], st[4 * g + 1], st[4 * g + 2], st[4 * g + 3]};
+                if (i + 1 < n) ahead(qs + (i + 1 & 3) * TILE, rowv + (i + 1 & 3) * 64);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const Frag<T> g = pack8<T>(st, u);
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) acc[d] = Mma<T>::run(w[u][d], g, acc[d]);
+                }
+            }
+            turn(n);
+        } else {
+            turn(0);
+            ahead(os, rowv + 32);
+            for (int i = 1; i <= n; ++i) {              // at tile i - 1
+                turn(i);
+                f32x16 ds[1], p;
+                const float* pt = ps + ((~i & 1) * 4 + pair) * 1024 + 4 * lane;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4 t = *reinterpret_cast<const f32x4*>(pt + 256 * g);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p[4 * g + e] = t[e];
+                }
+                Frag<T> w[2][DB];
+                const T* qt = qs + (i - 1 & 3) * TILE;
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) w[u][d] = lds.read_cols(qt, 16 * u, 32 * d);
+                __builtin_amdgcn_sched_barrier(0);
+                ds[0] = scores();
+                if (i < n) ahead(os + (i & 3) * TILE, rowv + (i & 3) * 64 + 32);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) ds[0][j] *= p[j];
+                cs.apply(ds, acc);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const Frag<T> g = pack8<T>(ds[0], u);
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) acc[d] = Mma<T>::run(w[u][d], g, acc[d]);
+                }
+            }
+        }
+    }
+    if (s >= a.S) return;
+    if (!there) {
+#pragma unroll
+        for (int b = 0; b < DB; ++b) acc[b] = splat16(0.f);
+    }
+    const int64_t row = ((int64_t)job.n * a.S + s) * hkv + job.hk;
+    const float by = first ? UNSHIFT : a.scale * UNSHIFT / cs.f;
+    void* o = a.o[first ? 1 : 0];
+    if (a.splits > 1)
+        store_col<float, DB>(static_cast<float*>(o) + job.split * a.numel + row * a.D, acc, by, a.D, lane);
+    else
+        store_col<T, DB>(static_cast<T*>(o) + row * a.D, acc, by, a.D, lane);
+}
+
 // out = sum of the splits' partials, in their order
 template <typename T>
 __global__ __launch_bounds__(256) void attn_sum_kernel(const float* __restrict__ part, int64_t numel, int splits, T* __restrict__ out) {
@@ -684,8 +899,11 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(const float* __restrict__
 // ---------------------------------------------------------------- host
 int pad_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
-// offsets within a tile of 64 rows are 32-bit byte offsets
-bool stride_ok(int64_t l) { return l >= 0 && l < (1ll << 23); }
+// 16-byte loads; offsets within a tile of 64 rows are 32-bit byte offsets; a row does not overlap the next
+bool rows_ok(const void* p, int64_t n, int64_t l, int64_t h, int D, int dtype) {
+    const int64_t e = dtype == DFSFM_F32 ? 4 : 8;
+    return !((uintptr_t)p & 15) && n % e == 0 && l % e == 0 && h % e == 0 && l >= D && l < (1ll << 23);
+}
 
 // Splits of the long axis (`length` rows of it, 256 a split at least).  512 workgroups run at a time (two a CU); as long as they number less
 // than eight such rounds the last one's idle places count, and the smallest number of splits that fills 85 % of the places is taken: 608
@@ -726,7 +944,7 @@ bool shape_ok(int N, int L, int S, int H, int Hkv, int D) {
 
 template <typename T, int DP>
 int forward_dp(Attn a, const Plan& p, T* out, hipStream_t st) {
-    constexpr int smem = 2 * KT * (PITCH<T, DP> + PITCH_T<T, DP>) * sizeof(T) + 2 * KT * 4;
+    constexpr int smem = 4 * Lds<T, DP>::TILE * sizeof(T);
     static dfsfm::SmemAttr attr;
     attr.ensure(reinterpret_cast<const void*>(&attn_forward_kernel<T, DP>), smem);
     a.tiles = p.tq;
@@ -745,7 +963,7 @@ template <typename T, int DP>
 int backward_dp(Attn a, const Plan& p, T* dq, T* dk, T* dv, float* part, hipStream_t st) {
     const int64_t rows = (int64_t)a.N * a.L * a.H, nq = rows * a.D, nk = (int64_t)a.N * a.S * (a.H / a.G) * a.D;
     if (rows > 0) {
-        constexpr int smem = 2 * KT * (PITCH<T, DP> + PITCH_T<T, DP>) * sizeof(T) + 2 * KT * 4;
+        constexpr int smem = 4 * Lds<T, DP>::TILE * sizeof(T);
         const bool few = a.S <= 2 * KT;        // one split: choose_splits cuts from 256 keys up
         a.tiles = p.tq;
         a.splits = p.dq;
@@ -766,15 +984,23 @@ int backward_dp(Attn a, const Plan& p, T* dq, T* dk, T* dv, float* part, hipStre
             hipLaunchKernelGGL((attn_sum_kernel<T>), dim3((unsigned)((nq / 4 + 255) / 256)), dim3(256), 0, st, part, nq, p.dq, dq);
     }
     if (nk > 0) {
-        constexpr int smem = 4 * KT * PITCH_T<T, DP> * sizeof(T) + 4 * KT * 4;
-        static dfsfm::SmemAttr attr;
-        attr.ensure(reinterpret_cast<const void*>(&attn_dkdv_kernel<T, DP>), smem);
         a.tiles = p.tk;
         a.splits = p.dkdv;
         a.numel = nk;
         a.o[0] = p.dkdv > 1 ? static_cast<void*>(part) : dk;
         a.o[1] = p.dkdv > 1 ? static_cast<void*>(part + p.dkdv * nk) : dv;
-        hipLaunchKernelGGL((attn_dkdv_kernel<T, DP>), dim3((unsigned)(p.heads * p.tk * p.dkdv)), dim3(256), smem, st, a);
+        const dim3 grid((unsigned)(p.heads * p.tk * p.dkdv));
+        if constexpr (DP == 128 && sizeof(T) == 2) {
+            constexpr int smem = 4 * Lds<T, DP>::TILE * sizeof(T) + 2 * 4 * 4096 + 4 * 2 * 32 * 4;
+            static dfsfm::SmemAttr attr;
+            attr.ensure(reinterpret_cast<const void*>(&attn_dkdv_pair_kernel<T>), smem);
+            hipLaunchKernelGGL((attn_dkdv_pair_kernel<T>), grid, dim3(512), smem, st, a);
+        } else {
+            constexpr int smem = 4 * Lds<T, DP>::TILE * sizeof(T) + 4 * KT * 4;
+            static dfsfm::SmemAttr attr;
+            attr.ensure(reinterpret_cast<const void*>(&attn_dkdv_kernel<T, DP>), smem);
+            hipLaunchKernelGGL((attn_dkdv_kernel<T, DP>), grid, dim3(256), smem, st, a);
+        }
         if (p.dkdv > 1) {
             const dim3 grid((unsigned)((nk / 4 + 255) / 256));
             hipLaunchKernelGGL((attn_sum_kernel<T>), grid, dim3(256), 0, st, part, nk, p.dkdv, dk);
@@ -813,7 +1039,8 @@ extern "C" int dfsfm_cross_attention(const void* q, int64_t qn, int64_t ql, int6
     if (N == 0 || L == 0 || H == 0) return DFSFM_OK;
     if (!q || !out || !lse || (S > 0 && (!k || !v)) || N < 0 || L < 0 || S < 0 || H < 0 || !(scale > 0.f)) return DFSFM_E_BADARG;
     if (!shape_ok(N, L, S, H, Hkv, D)) return DFSFM_E_UNSUPPORTED;
-    if (!stride_ok(ks) || !stride_ok(vs)) return DFSFM_E_UNSUPPORTED;
+    if (dtype < DFSFM_F32 || dtype > DFSFM_F16 || !rows_ok(q, qn, ql, qh, D, dtype) || ((uintptr_t)out & 15)) return DFSFM_E_UNSUPPORTED;
+    if (S > 0 && (!rows_ok(k, kn, ks, kh, D, dtype) || !rows_ok(v, vn, vs, vh, D, dtype))) return DFSFM_E_UNSUPPORTED;
     if (workspace_bytes < dfsfm_cross_attention_workspace(N, L, S, H, Hkv, D)) return DFSFM_E_WORKSPACE;
     Attn a{};
     a.q = {q, qn, ql, qh};
@@ -852,7 +1079,10 @@ extern "C" int dfsfm_cross_attention_backward(const void* dout, int64_t gn, int6
     if (N < 0 || L < 0 || S < 0 || H < 0 || !(scale > 0.f)) return DFSFM_E_BADARG;
     if ((L > 0 && (!dout || !q || !out || !lse || !dq)) || (S > 0 && (!k || !v || !dk || !dv))) return DFSFM_E_BADARG;
     if (!shape_ok(N, L, S, H, Hkv, D)) return DFSFM_E_UNSUPPORTED;
-    if (!stride_ok(ks) || !stride_ok(vs) || !stride_ok(ql) || !stride_ok(gl)) return DFSFM_E_UNSUPPORTED;
+    if (dtype < DFSFM_F32 || dtype > DFSFM_F16 || (((uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15)) return DFSFM_E_UNSUPPORTED;
+    if (L > 0 && (!rows_ok(q, qn, ql, qh, D, dtype) || !rows_ok(dout, gn, gl, gh, D, dtype) || !rows_ok(out, on, ol, oh, D, dtype)))
+        return DFSFM_E_UNSUPPORTED;
+    if (S > 0 && (!rows_ok(k, kn, ks, kh, D, dtype) || !rows_ok(v, vn, vs, vh, D, dtype))) return DFSFM_E_UNSUPPORTED;
     if (workspace_bytes < dfsfm_cross_attention_backward_workspace(N, L, S, H, Hkv, D)) return DFSFM_E_WORKSPACE;
     Attn a{};
     a.q = {q, qn, ql, qh};

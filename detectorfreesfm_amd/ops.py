@@ -1857,9 +1857,13 @@ def rotary_backward(dy, positions, inv_freq, amplitude=1.0, axes=1, interleaved=
 
 
 def _heads(t):
-    """[N, L, H, D] heads as the kernels read them: a unit channel stride, tokens less than 2^23 elements apart."""
-    s = t.stride()
-    return t if s[3] == 1 and s[1] < 1 << 23 else t.contiguous()
+    """[N, L, H, D] heads as the kernels read them: a unit channel stride, rows on 16-byte boundaries, at least D and less than 2^23
+    elements apart; anything else is copied."""
+    n, l, h, c = t.stride()
+    e = 16 // t.element_size() - 1
+    if c == 1 and t.shape[3] <= l < 1 << 23 and not (n | l | h) & e and not t.data_ptr() & 15:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _attention_args(what, q, k, v, kv_lens, kv_mask, scale, more=()):

@@ -245,8 +245,8 @@ int dfsfm_rotary(const void* x, int64_t xn, int64_t xl, int64_t xh, void* y, int
                  const int64_t* positions, int64_t pn, int64_t pl, int64_t pa, const double* inv_freq, int pairs, int axes, int interleaved,
                  int backward, float amplitude, int N, int64_t L, int H, int D, int dtype, void* stream);
 
-/* Softmax attention of q [N, L, H, D] over an encoder's states k, v [N, S, Hkv, D] of another length (element strides n, length, head, the length's below 2^23;
- * unit channel stride; any alignment; D a multiple of 8 up to 128; H a multiple of Hkv, query head h reads key head h / (H / Hkv)):
+/* Softmax attention of q [N, L, H, D] over an encoder's states k, v [N, S, Hkv, D] of another length (element strides n, length, head; unit
+ * channel stride; rows on 16-byte boundaries, length strides from D to below 2^23; D a multiple of 8 up to 128; H a multiple of Hkv, query head h reads key head h / (H / Hkv)):
  * out [N, L, H, D] dense = softmax(scale * q k^T) v and lse [N, H, L] = log sum exp(scale * q k^T) in fp32, over the keys s < kv_lens[n]
  * (int32, clamped to 0 .. S; null: all) with kv_mask[n, s] != 0 (uint8, dense [N, S]; null: all).  What k and v hold elsewhere is not
  * looked at, NaN included.  A query without keys gets out = 0, lse = -inf.  scale > 0. */
