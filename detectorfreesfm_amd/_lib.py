@@ -129,11 +129,11 @@ SIGNATURES = [
     ("dfsfm_rotary", c_int,
      [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int, c_int,
       c_int, c_int, c_float, c_int, c_int64, c_int, c_int, c_int, c_void_p]),
-    ("dfsfm_cross_attention_workspace", c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    ("dfsfm_cross_attention_workspace", c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     ("dfsfm_cross_attention", c_int,
      [c_void_p, c_int64, c_int64, c_int64] * 3 + [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float,
       c_int, c_void_p, c_size_t, c_void_p]),
-    ("dfsfm_cross_attention_backward_workspace", c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    ("dfsfm_cross_attention_backward_workspace", c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     ("dfsfm_cross_attention_backward", c_int,
      [c_void_p, c_int64, c_int64, c_int64] * 5 + [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
       c_int, c_int, c_float, c_int, c_void_p, c_size_t, c_void_p]),

@@ -163,6 +163,25 @@ struct Job {
         n = head / hkv;
         hk = head % hkv;
     }
+    // The same for tiles of `rows` keys, the tiles with keys of every sequence first: workgroups go to XCDs by their number, so tiles that
+    // have nothing to do must not lie between the others (4 x 6400 ragged keys: XCDs with four rounds of work beside ones with three).
+    __device__ __forceinline__ Job(const Attn& a, int rows) : Job(a) {
+        if (!a.lens || a.N > 64) return;
+        const int hkv = a.H / a.G, per = hkv * a.splits;
+        unsigned id = blockIdx.x;
+        for (int pass = 0; pass < 2; ++pass)
+            for (int i = 0; i < a.N; ++i) {
+                const int with = (min(max(a.lens[i], 0), a.S) + rows - 1) / rows, tiles = pass ? a.tiles - with : with;
+                if (id < (unsigned)(tiles * per)) {
+                    n = i;
+                    tile = (pass ? with : 0) + id % tiles;
+                    hk = id / tiles % hkv;
+                    split = id / tiles / hkv;
+                    return;
+                }
+                id -= tiles * per;
+            }
+    }
 };
 
 __device__ __forceinline__ int valid_len(const Attn& a, int n) { return a.lens ? min(max(a.lens[n], 0), a.S) : a.S; }
@@ -608,20 +627,31 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
         store_col<T, DB>(static_cast<T*>(a.o[0]) + row * a.D, acc, f, a.D, lane);
 }
 
-// dk and dv: 4 waves x 32 keys a workgroup, tiles of 64 rows of q and dout, both read both ways.
+// dk and dv: NW waves x 32 keys a workgroup, tiles of 64 rows of q and dout, both read both ways.
+//
+// NW is 4, two workgroups a CU, where a wave's K, V, dk and dv leave room for two waves a SIMD.  At D = 128 in 16 bits they are 192 registers
+// before the first score; there NW is 8, one workgroup a CU, and V stays in LDS (64 KB for 256 keys), read again for every tile.
+// 4 x 4800 x 6400 (ragged) x 16 heads bf16 takes 1.21 - 1.31 ms; with V in registers, four waves and one wave a SIMD 2.3; with the two halves
+// of the work on two waves that pass p through LDS 1.7; as two launches, one product made twice, 1.8.
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void attn_dkdv_kernel(const Attn a) {
+constexpr int KEY_WAVES = DP == 128 && sizeof(T) == 2 ? 8 : 4;
+
+template <typename T, int DP>
+__global__ __launch_bounds__((64 * KEY_WAVES<T, DP>), (KEY_WAVES<T, DP> / 4)) void attn_dkdv_kernel(const Attn a) {
+    constexpr int NW = KEY_WAVES<T, DP>, THREADS = 64 * NW;
+    constexpr bool VLDS = NW == 8;
     constexpr int DB = DP / 32, KS = DP / 16, TILE = Lds<T, DP>::TILE;
     // p of fp16 tensors times 2^14: a power of two that keeps weights down to 2^-28 exact and 1 in range
     constexpr float SHIFT = __is_same(T, f16) ? 14.f : 0.f, UNSHIFT = __is_same(T, f16) ? 1.f / 16384.f : 1.f;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* qs = reinterpret_cast<T*>(smem);
     T* os = qs + 2 * TILE;
-    float* rowv = reinterpret_cast<float*>(os + 2 * TILE);                // [2][2][64]: -lse / scale, -delta
-    const Job job(a);
+    T* vs = os + 2 * TILE;                                                // VLDS: the workgroup's keys
+    float* rowv = reinterpret_cast<float*>(vs + (VLDS ? NW * 32 * DP : 0));      // [2][2][64]: -lse / scale, -delta
+    const Job job(a, NW * 32);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hkv = a.H / a.G;
     const Lds<T, DP> lds(lane);
-    const int s = job.tile * 128 + wave * 32 + (lane & 31);
+    const int s = job.tile * (NW * 32) + wave * 32 + (lane & 31);
     const int len = valid_len(a, job.n);
     bool there = s < len;
     if (a.mask) there = there && a.mask[(int64_t)job.n * a.S + min(s, a.S - 1)] != 0;
@@ -629,19 +659,19 @@ __global__ __launch_bounds__(256) void attn_dkdv_kernel(const Attn a) {
     const int lt = (a.L + KT - 1) / KT, per = (lt * a.G + a.splits - 1) / a.splits;
     const int beg = min(lt * a.G, job.split * per), end = min(lt * a.G, beg + per);
 
-    Frag<T> kf[KS], vf[KS];
+    Frag<T> kf[KS], vf[VLDS ? 1 : KS];
     const T* kp = static_cast<const T*>(a.k.p) + job.n * a.k.n + (int64_t)min(s, a.S - 1) * a.k.l + job.hk * a.k.h;
     const T* vp = static_cast<const T*>(a.v.p) + job.n * a.v.n + (int64_t)min(s, a.S - 1) * a.v.l + job.hk * a.v.h;
 #pragma unroll
     for (int x = 0; x < KS; ++x) {
         const int c = 16 * x + 8 * (lane >> 5);
         kf[x] = there && c < a.D ? load8<T>(kp + c) : zero_frag<T>();
-        vf[x] = there && c < a.D ? load8<T>(vp + c) : zero_frag<T>();
+        if constexpr (!VLDS) vf[x] = there && c < a.D ? load8<T>(vp + c) : zero_frag<T>();
     }
     const T* qb = static_cast<const T*>(a.q.p) + job.n * a.q.n + job.hk * a.G * a.q.h;
     const T* ob = static_cast<const T*>(a.dout.p) + job.n * a.dout.n + job.hk * a.G * a.dout.h;
     const int64_t vec = ((int64_t)job.n * a.H + job.hk * a.G) * a.L;
-    const Dma<T, DP, KT, 256> dq(a.q.l, a.D), dd(a.dout.l, a.D);
+    const Dma<T, DP, KT, THREADS> dq(a.q.l, a.D), dd(a.dout.l, a.D);
     float rv = 0.f;                         // threads 0..63: lse of a row, 64..127: delta
     const float inv_scale = 1.f / a.scale;
     int rows = 0;                           // rows of the tile in flight
@@ -661,7 +691,15 @@ __global__ __launch_bounds__(256) void attn_dkdv_kernel(const Attn a) {
     ColumnScale<T, DB> cs;
     const float c = a.scale * LOG2E;
     const bool any = __syncthreads_or(there);
-    if (any && beg < end) fetch(beg, 0);
+    if (any && beg < end) {
+        if constexpr (VLDS) {               // masked keys come as they are: a key's column is its own, and dropped at the end
+            const int s0 = job.tile * (NW * 32);
+            const Dma<T, DP, NW * 32, THREADS> dv(a.v.l, a.D);
+            dv.issue(static_cast<const T*>(a.v.p) + job.n * a.v.n + job.hk * a.v.h + s0 * a.v.l, len - s0, vs);
+        }
+        fetch(beg, 0);
+    }
+    const bool mine = __ballot(there) != 0;
     int buf = 0;
     for (int it = beg; any && it < end; ++it, buf ^= 1) {
         T* qt = qs + buf * TILE;
@@ -675,7 +713,8 @@ __global__ __launch_bounds__(256) void attn_dkdv_kernel(const Attn a) {
         }
         __syncthreads();
         if (it + 1 < end) fetch(it + 1, buf ^ 1);
-#pragma unroll
+        if (!mine) continue;
+#pragma unroll(VLDS ? 1 : 2)
         for (int b = 0; b < 2; ++b) {
             f32x16 st = rows16(vt + 32 * b, lane);
             f32x16 ds[1];
@@ -683,7 +722,7 @@ __global__ __launch_bounds__(256) void attn_dkdv_kernel(const Attn a) {
 #pragma unroll
             for (int x = 0; x < KS; ++x) {
                 st = Mma<T>::run(lds.read_rows(qt, 32 * b, 16 * x), kf[x], st);
-                ds[0] = Mma<T>::run(lds.read_rows(ot, 32 * b, 16 * x), vf[x], ds[0]);
+                ds[0] = Mma<T>::run(lds.read_rows(ot, 32 * b, 16 * x), VLDS ? lds.read_rows(vs, 32 * wave, 16 * x) : vf[VLDS ? 0 : x], ds[0]);
             }
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
@@ -691,6 +730,7 @@ __global__ __launch_bounds__(256) void attn_dkdv_kernel(const Attn a) {
                 ds[0][j] *= st[j];
             }
             cs.apply(ds, dk);
+            if constexpr (VLDS) __builtin_amdgcn_sched_barrier(0);       // with the loop above not unrolled: no register spilled
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const Frag<T> p = pack8<T>(st, u), g = pack8<T>(ds[0], u);
@@ -718,169 +758,6 @@ __global__ __launch_bounds__(256) void attn_dkdv_kernel(const Attn a) {
     }
 }
 
-// dk and dv for D = 128 in 16 bits: one wave's K, V, dk and dv need 192 registers before the first score, which leaves one wave a SIMD and
-// nothing to run beside its exponentials.  Here two waves share 32 keys: waves 0 .. 3 make p and dv, waves 4 .. 7 dp, ds and dk, half of the
-// products each and half of the registers.  p goes through LDS in 32 bits, lane to lane in accumulator order, one tile behind: while a first
-// wave is at tile i, its partner is at tile i - 1.  Every operand is on its way from LDS a product ahead: a tile's score operands while the
-// tile before is accumulated, the transposed ones before the exponentials.  Tiles are 32 rows, four in LDS: i - 1 .. i + 1 being read, i + 2
-// being written.
-template <typename T>
-__global__ __launch_bounds__(512, 2) void attn_dkdv_pair_kernel(const Attn a) {
-    constexpr int DP = 128, DB = DP / 32, KS = DP / 16, QT = 32, TILE = Lds<T, DP>::TILE / 2;
-    constexpr float SHIFT = __is_same(T, f16) ? 14.f : 0.f, UNSHIFT = __is_same(T, f16) ? 1.f / 16384.f : 1.f;
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    T* qs = reinterpret_cast<T*>(smem);                                   // [4][32][DP]
-    T* os = qs + 4 * TILE;
-    float* ps = reinterpret_cast<float*>(os + 4 * TILE);                  // [2][4 pairs][4][64 lanes] x 4
-    float* rowv = ps + 2 * 4 * 1024;                                      // [4][2][32]: -lse / scale, -delta
-    const Job job(a);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pair = wave & 3, hkv = a.H / a.G;
-    const bool first = wave < 4;
-    const Lds<T, DP> lds(lane);
-    const int s = job.tile * 128 + pair * 32 + (lane & 31);
-    const int len = valid_len(a, job.n);
-    bool there = s < len;
-    if (a.mask) there = there && a.mask[(int64_t)job.n * a.S + min(s, a.S - 1)] != 0;
-    const int lt = (a.L + QT - 1) / QT, per = (lt * a.G + a.splits - 1) / a.splits;
-    const int beg = min(lt * a.G, job.split * per), end = min(lt * a.G, beg + per);
-
-    Frag<T> kv[KS];                         // K of a first wave, V of a second
-    const Tensor& own = first ? a.k : a.v;
-    const T* kp = static_cast<const T*>(own.p) + job.n * own.n + (int64_t)min(s, a.S - 1) * own.l + job.hk * own.h;
-#pragma unroll
-    for (int x = 0; x < KS; ++x) {
-        const int c = 16 * x + 8 * (lane >> 5);
-        kv[x] = there && c < a.D ? load8<T>(kp + c) : zero_frag<T>();
-    }
-    const T* qb = static_cast<const T*>(a.q.p) + job.n * a.q.n + job.hk * a.G * a.q.h;
-    const T* ob = static_cast<const T*>(a.dout.p) + job.n * a.dout.n + job.hk * a.G * a.dout.h;
-    const int64_t vec = ((int64_t)job.n * a.H + job.hk * a.G) * a.L;
-    const Dma<T, DP, QT, 512> dq(a.q.l, a.D), dd(a.dout.l, a.D);
-    const float inv_scale = 1.f / a.scale;
-    float rv = 0.f;                         // threads 0..31: lse of a row, 32..63: delta
-    int rows = 0;                           // rows of the tile in flight
-    auto fetch = [&](int i) {               // tile beg + i
-        const int it = beg + i, g = it / lt, l0 = (it - g * lt) * QT;
-        rows = a.L - l0;
-        dq.issue(qb + g * a.q.h + l0 * a.q.l, rows, qs + (i & 3) * TILE);
-        dd.issue(ob + g * a.dout.h + l0 * a.dout.l, rows, os + (i & 3) * TILE);
-        if (threadIdx.x < 64) rv = (threadIdx.x < 32 ? a.lse : a.delta)[vec + (int64_t)g * a.L + l0 + min((int)threadIdx.x & 31, rows - 1)];
-    };
-    auto put = [&](int i) {                 // its row values, once they are here
-        if (threadIdx.x < 64) {
-            const bool in = (int)(threadIdx.x & 31) < rows;
-            rowv[(i & 3) * 64 + threadIdx.x] = threadIdx.x < 32 ? (in && rv != NEG ? -rv * inv_scale : NEG) : (in ? -rv : 0.f);
-        }
-    };
-    f32x16 acc[DB];                         // dv of a first wave, dk of a second
-#pragma unroll
-    for (int b = 0; b < DB; ++b) acc[b] = splat16(0.f);
-    ColumnScale<T, DB> cs;
-    const float c = a.scale * LOG2E;
-    Frag<T> f[KS];                          // score operands of the tile at hand
-    f32x16 start;
-    auto ahead = [&](const T* tile, const float* from) {
-#pragma unroll
-        for (int x = 0; x < KS; ++x) f[x] = lds.read_rows(tile, 0, 16 * x);
-        start = rows16(from, lane);
-    };
-    auto scores = [&]() {
-        f32x16 st = start;
-#pragma unroll
-        for (int x = 0; x < KS; ++x) st = Mma<T>::run(f[x], kv[x], st);
-        return st;
-    };
-    const bool any = __syncthreads_or(there) && beg < end;
-    if (any) {
-        const int n = end - beg;
-        fetch(0);
-        dma_landed();
-        put(0);
-        if (n > 1) fetch(1);
-        // Past the barrier tile i + 1 is in LDS, and tile i + 2 leaves memory for the place of tile i - 2, whose readers are done.
-        auto turn = [&](int i) {
-            dma_landed();
-            if (i + 1 < n) put(i + 1);
-            __syncthreads();
-            if (i + 2 < n) fetch(i + 2);
-        };
-        // both halves pass n + 1 barriers
-        if (first) {
-            for (int i = 0; i < n; ++i) {
-                turn(i);
-                if (i == 0) ahead(qs, rowv);
-                f32x16 st = scores();
-                Frag<T> w[2][DB];
-                const T* ot = os + (i & 3) * TILE;
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) w[u][d] = lds.read_cols(ot, 16 * u, 32 * d);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) st[j] = __builtin_amdgcn_exp2f(fmaf(st[j], c, SHIFT));
-                float* pt = ps + ((i & 1) * 4 + pair) * 1024 + 4 * lane;
-#pragma unroll
-                for (int g = 0; g < 4; ++g) *reinterpret_cast<f32x4*>(pt + 256 * g) = f32x4{st[4 * g], st[4 * g + 1], st[4 * g + 2], st[4 * g + 3]};
-                if (i + 1 < n) ahead(qs + (i + 1 & 3) * TILE, rowv + (i + 1 & 3) * 64);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const Frag<T> g = pack8<T>(st, u);
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) acc[d] = Mma<T>::run(w[u][d], g, acc[d]);
-                }
-            }
-            turn(n);
-        } else {
-            turn(0);
-            ahead(os, rowv + 32);
-            for (int i = 1; i <= n; ++i) {              // at tile i - 1
-                turn(i);
-                f32x16 ds[1], p;
-                const float* pt = ps + ((~i & 1) * 4 + pair) * 1024 + 4 * lane;
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f32x4 t = *reinterpret_cast<const f32x4*>(pt + 256 * g);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) p[4 * g + e] = t[e];
-                }
-                Frag<T> w[2][DB];
-                const T* qt = qs + (i - 1 & 3) * TILE;
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) w[u][d] = lds.read_cols(qt, 16 * u, 32 * d);
-                __builtin_amdgcn_sched_barrier(0);
-                ds[0] = scores();
-                if (i < n) ahead(os + (i & 3) * TILE, rowv + (i & 3) * 64 + 32);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) ds[0][j] *= p[j];
-                cs.apply(ds, acc);
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const Frag<T> g = pack8<T>(ds[0], u);
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) acc[d] = Mma<T>::run(w[u][d], g, acc[d]);
-                }
-            }
-        }
-    }
-    if (s >= a.S) return;
-    if (!there) {
-#pragma unroll
-        for (int b = 0; b < DB; ++b) acc[b] = splat16(0.f);
-    }
-    const int64_t row = ((int64_t)job.n * a.S + s) * hkv + job.hk;
-    const float by = first ? UNSHIFT : a.scale * UNSHIFT / cs.f;
-    void* o = a.o[first ? 1 : 0];
-    if (a.splits > 1)
-        store_col<float, DB>(static_cast<float*>(o) + job.split * a.numel + row * a.D, acc, by, a.D, lane);
-    else
-        store_col<T, DB>(static_cast<T*>(o) + row * a.D, acc, by, a.D, lane);
-}
-
 // out = sum of the splits' partials, in their order
 template <typename T>
 __global__ __launch_bounds__(256) void attn_sum_kernel(const float* __restrict__ part, int64_t numel, int splits, T* __restrict__ out) {
@@ -905,16 +782,16 @@ bool rows_ok(const void* p, int64_t n, int64_t l, int64_t h, int D, int dtype) {
     return !((uintptr_t)p & 15) && n % e == 0 && l % e == 0 && h % e == 0 && l >= D && l < (1ll << 23);
 }
 
-// Splits of the long axis (`length` rows of it, 256 a split at least).  512 workgroups run at a time (two a CU); as long as they number less
-// than eight such rounds the last one's idle places count, and the smallest number of splits that fills 85 % of the places is taken: 608
+// Splits of the long axis (`length` rows of it, 256 a split at least).  `slots` workgroups run at a time (512: two a CU); as long as they
+// number less than eight such rounds the last one's idle places count, and the smallest number of splits that fills 85 % of the places is taken: 608
 // workgroups of the forward pass 2 x 4800 x 10816 x 8 x 32 fp32 take 1.21 ms, three splits of each 0.98 with the join.
-int choose_splits(int64_t groups, int64_t length) {
-    if (groups <= 0 || groups >= 4096) return 1;
+int choose_splits(int64_t groups, int64_t length, int slots) {
+    if (groups <= 0 || groups >= 8 * slots) return 1;
     const int64_t most = length / 256 < 256 ? length / 256 : 256;
     int best = 1;
     double fill = 0;
     for (int s = 1; s <= most || s == 1; ++s) {
-        const int64_t n = groups * s, places = (n + 511) / 512 * 512;
+        const int64_t n = groups * s, places = (n + slots - 1) / slots * slots;
         const double f = (double)n / (double)places;
         if (f > fill + 0.02) fill = f, best = s;
         if (fill >= 0.85) break;
@@ -924,13 +801,14 @@ int choose_splits(int64_t groups, int64_t length) {
 
 struct Plan {
     int heads, tq, tk, fwd, dq, dkdv;       // row tiles, key tiles, splits
-    Plan(int N, int L, int S, int H, int Hkv) {
+    Plan(int N, int L, int S, int H, int Hkv, int D, int dtype) {
         heads = N * Hkv;
         const int64_t R = (int64_t)L * (H / Hkv);
+        const int dp = pad_dim(D), keys = 32 * (dtype == DFSFM_F32 ? KEY_WAVES<float, 128> : dp == 128 ? KEY_WAVES<bf16, 128> : KEY_WAVES<bf16, 32>);
         tq = (int)((R + 127) / 128);
-        tk = (S + 127) / 128;
-        fwd = dq = choose_splits((int64_t)heads * tq, S);
-        dkdv = choose_splits((int64_t)heads * tk, R);
+        tk = (S + keys - 1) / keys;
+        fwd = dq = choose_splits((int64_t)heads * tq, S, 512);
+        dkdv = choose_splits((int64_t)heads * tk, R, keys == 256 ? 256 : 512);
     }
 };
 
@@ -989,18 +867,11 @@ int backward_dp(Attn a, const Plan& p, T* dq, T* dk, T* dv, float* part, hipStre
         a.numel = nk;
         a.o[0] = p.dkdv > 1 ? static_cast<void*>(part) : dk;
         a.o[1] = p.dkdv > 1 ? static_cast<void*>(part + p.dkdv * nk) : dv;
-        const dim3 grid((unsigned)(p.heads * p.tk * p.dkdv));
-        if constexpr (DP == 128 && sizeof(T) == 2) {
-            constexpr int smem = 4 * Lds<T, DP>::TILE * sizeof(T) + 2 * 4 * 4096 + 4 * 2 * 32 * 4;
-            static dfsfm::SmemAttr attr;
-            attr.ensure(reinterpret_cast<const void*>(&attn_dkdv_pair_kernel<T>), smem);
-            hipLaunchKernelGGL((attn_dkdv_pair_kernel<T>), grid, dim3(512), smem, st, a);
-        } else {
-            constexpr int smem = 4 * Lds<T, DP>::TILE * sizeof(T) + 4 * KT * 4;
-            static dfsfm::SmemAttr attr;
-            attr.ensure(reinterpret_cast<const void*>(&attn_dkdv_kernel<T, DP>), smem);
-            hipLaunchKernelGGL((attn_dkdv_kernel<T, DP>), grid, dim3(256), smem, st, a);
-        }
+        constexpr int NW = KEY_WAVES<T, DP>;
+        constexpr int smem = (4 * Lds<T, DP>::TILE + (NW == 8 ? NW * 32 * DP : 0)) * sizeof(T) + 4 * KT * 4;
+        static dfsfm::SmemAttr attr;
+        attr.ensure(reinterpret_cast<const void*>(&attn_dkdv_kernel<T, DP>), smem);
+        hipLaunchKernelGGL((attn_dkdv_kernel<T, DP>), dim3((unsigned)(p.heads * p.tk * p.dkdv)), dim3(64 * NW), smem, st, a);
         if (p.dkdv > 1) {
             const dim3 grid((unsigned)((nk / 4 + 255) / 256));
             hipLaunchKernelGGL((attn_sum_kernel<T>), grid, dim3(256), 0, st, part, nk, p.dkdv, dk);
@@ -1026,9 +897,9 @@ int backward_any(const Attn& a, const Plan& p, void* dq, void* dk, void* dv, flo
 
 }  // namespace
 
-extern "C" size_t dfsfm_cross_attention_workspace(int N, int L, int S, int H, int Hkv, int D) {
+extern "C" size_t dfsfm_cross_attention_workspace(int N, int L, int S, int H, int Hkv, int D, int dtype) {
     if (N <= 0 || L <= 0 || S < 0 || H <= 0 || !shape_ok(N, L, S, H, Hkv, D)) return 0;
-    const Plan p(N, L, S, H, Hkv);
+    const Plan p(N, L, S, H, Hkv, D, dtype);
     return p.fwd > 1 ? (size_t)p.fwd * N * L * H * (D + 2) * sizeof(float) : 0;
 }
 
@@ -1041,7 +912,7 @@ extern "C" int dfsfm_cross_attention(const void* q, int64_t qn, int64_t ql, int6
     if (!shape_ok(N, L, S, H, Hkv, D)) return DFSFM_E_UNSUPPORTED;
     if (dtype < DFSFM_F32 || dtype > DFSFM_F16 || !rows_ok(q, qn, ql, qh, D, dtype) || ((uintptr_t)out & 15)) return DFSFM_E_UNSUPPORTED;
     if (S > 0 && (!rows_ok(k, kn, ks, kh, D, dtype) || !rows_ok(v, vn, vs, vh, D, dtype))) return DFSFM_E_UNSUPPORTED;
-    if (workspace_bytes < dfsfm_cross_attention_workspace(N, L, S, H, Hkv, D)) return DFSFM_E_WORKSPACE;
+    if (workspace_bytes < dfsfm_cross_attention_workspace(N, L, S, H, Hkv, D, dtype)) return DFSFM_E_WORKSPACE;
     Attn a{};
     a.q = {q, qn, ql, qh};
     a.k = {k, kn, ks, kh};
@@ -1051,7 +922,7 @@ extern "C" int dfsfm_cross_attention(const void* q, int64_t qn, int64_t ql, int6
     a.lse = lse;
     a.N = N, a.L = L, a.S = S, a.H = H, a.G = H / Hkv, a.D = D, a.scale = scale;
     a.numel = (int64_t)N * L * H * D;
-    const Plan p(N, L, S, H, Hkv);
+    const Plan p(N, L, S, H, Hkv, D, dtype);
     a.o[0] = workspace;
     a.ml = static_cast<float*>(workspace) + p.fwd * a.numel;
     hipStream_t st = static_cast<hipStream_t>(stream_);
@@ -1061,9 +932,9 @@ extern "C" int dfsfm_cross_attention(const void* q, int64_t qn, int64_t ql, int6
     return DFSFM_E_UNSUPPORTED;
 }
 
-extern "C" size_t dfsfm_cross_attention_backward_workspace(int N, int L, int S, int H, int Hkv, int D) {
+extern "C" size_t dfsfm_cross_attention_backward_workspace(int N, int L, int S, int H, int Hkv, int D, int dtype) {
     if (N <= 0 || L < 0 || S < 0 || H <= 0 || !shape_ok(N, L, S, H, Hkv, D)) return 0;
-    const Plan p(N, L, S, H, Hkv);
+    const Plan p(N, L, S, H, Hkv, D, dtype);
     const size_t nq = (size_t)N * L * H, nk = (size_t)N * S * Hkv * D;
     const size_t a = p.dq > 1 ? p.dq * nq * D : 0, b = p.dkdv > 1 ? 2 * p.dkdv * nk : 0;
     return (nq + (a > b ? a : b)) * sizeof(float);
@@ -1083,7 +954,7 @@ extern "C" int dfsfm_cross_attention_backward(const void* dout, int64_t gn, int6
     if (L > 0 && (!rows_ok(q, qn, ql, qh, D, dtype) || !rows_ok(dout, gn, gl, gh, D, dtype) || !rows_ok(out, on, ol, oh, D, dtype)))
         return DFSFM_E_UNSUPPORTED;
     if (S > 0 && (!rows_ok(k, kn, ks, kh, D, dtype) || !rows_ok(v, vn, vs, vh, D, dtype))) return DFSFM_E_UNSUPPORTED;
-    if (workspace_bytes < dfsfm_cross_attention_backward_workspace(N, L, S, H, Hkv, D)) return DFSFM_E_WORKSPACE;
+    if (workspace_bytes < dfsfm_cross_attention_backward_workspace(N, L, S, H, Hkv, D, dtype)) return DFSFM_E_WORKSPACE;
     Attn a{};
     a.q = {q, qn, ql, qh};
     a.k = {k, kn, ks, kh};
@@ -1094,7 +965,7 @@ extern "C" int dfsfm_cross_attention_backward(const void* dout, int64_t gn, int6
     a.mask = kv_mask;
     a.lse = const_cast<float*>(lse);
     a.N = N, a.L = L, a.S = S, a.H = H, a.G = H / Hkv, a.D = D, a.scale = scale;
-    const Plan p(N, L, S, H, Hkv);
+    const Plan p(N, L, S, H, Hkv, D, dtype);
     a.delta = static_cast<float*>(workspace);
     float* part = a.delta + (int64_t)N * L * H;
     hipStream_t st = static_cast<hipStream_t>(stream_);

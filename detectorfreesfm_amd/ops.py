@@ -1913,7 +1913,7 @@ def cross_attention(q, k, v, kv_lens=None, kv_mask=None, scale=None):
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty((N, H, L), dtype=torch.float32)
     lib = _lib.lib()
-    nbytes = lib.dfsfm_cross_attention_workspace(N, L, S, H, Hkv, D)
+    nbytes = lib.dfsfm_cross_attention_workspace(N, L, S, H, Hkv, D, code)
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     rc = lib.dfsfm_cross_attention(*_heads_ptr(q), *_heads_ptr(k), *_heads_ptr(v), lens, mask, out.data_ptr(), lse.data_ptr(), N, L, S, H, Hkv,
                                    D, scale, code, ws.data_ptr() if nbytes else None, nbytes, _raw_stream(q.get_device()))
@@ -1937,7 +1937,7 @@ def cross_attention_backward(dout, q, k, v, out, lse, kv_lens=None, kv_mask=None
     dq = torch.empty_like(q, memory_format=torch.contiguous_format)
     dk, dv = torch.empty_like(k, memory_format=torch.contiguous_format), torch.empty_like(v, memory_format=torch.contiguous_format)
     lib = _lib.lib()
-    nbytes = lib.dfsfm_cross_attention_backward_workspace(N, L, S, H, Hkv, D)
+    nbytes = lib.dfsfm_cross_attention_backward_workspace(N, L, S, H, Hkv, D, code)
     ws = q.new_empty(nbytes, dtype=torch.uint8)
     rc = lib.dfsfm_cross_attention_backward(*_heads_ptr(dout), *_heads_ptr(q), *_heads_ptr(k), *_heads_ptr(v), *_heads_ptr(out),
                                             lse.data_ptr(), lens, mask, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), N, L, S, H, Hkv, D, scale,

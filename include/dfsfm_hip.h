@@ -250,7 +250,7 @@ int dfsfm_rotary(const void* x, int64_t xn, int64_t xl, int64_t xh, void* y, int
  * out [N, L, H, D] dense = softmax(scale * q k^T) v and lse [N, H, L] = log sum exp(scale * q k^T) in fp32, over the keys s < kv_lens[n]
  * (int32, clamped to 0 .. S; null: all) with kv_mask[n, s] != 0 (uint8, dense [N, S]; null: all).  What k and v hold elsewhere is not
  * looked at, NaN included.  A query without keys gets out = 0, lse = -inf.  scale > 0. */
-size_t dfsfm_cross_attention_workspace(int N, int L, int S, int H, int Hkv, int D);
+size_t dfsfm_cross_attention_workspace(int N, int L, int S, int H, int Hkv, int D, int dtype);
 int dfsfm_cross_attention(const void* q, int64_t qn, int64_t ql, int64_t qh, const void* k, int64_t kn, int64_t ks, int64_t kh,
                           const void* v, int64_t vn, int64_t vs, int64_t vh, const int* kv_lens, const uint8_t* kv_mask, void* out,
                           float* lse, int N, int L, int S, int H, int Hkv, int D, float scale, int dtype, void* workspace,
@@ -259,7 +259,7 @@ int dfsfm_cross_attention(const void* q, int64_t qn, int64_t ql, int64_t qh, con
 /* Its gradient for dout [N, L, H, D] from the forward pass's out and lse: dq [N, L, H, D], dk, dv [N, S, Hkv, D], dense, in the dtype; the
  * gradients of shared key heads are sums over their query heads; keys that are not there get zeros.  kv_lens, kv_mask and scale are the
  * forward pass's. */
-size_t dfsfm_cross_attention_backward_workspace(int N, int L, int S, int H, int Hkv, int D);
+size_t dfsfm_cross_attention_backward_workspace(int N, int L, int S, int H, int Hkv, int D, int dtype);
 int dfsfm_cross_attention_backward(const void* dout, int64_t gn, int64_t gl, int64_t gh, const void* q, int64_t qn, int64_t ql, int64_t qh,
                                    const void* k, int64_t kn, int64_t ks, int64_t kh, const void* v, int64_t vn, int64_t vs, int64_t vh,
                                    const void* out, int64_t on, int64_t ol, int64_t oh, const float* lse, const int* kv_lens,
