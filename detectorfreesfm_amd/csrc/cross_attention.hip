@@ -22,7 +22,6 @@ using dfsfm::check_launch;
 using dfsfm::mfma32_row;
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr int KT = 64;                     // rows of a staged tile
 constexpr float NEG = -INFINITY;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -51,22 +50,94 @@ struct Mma<float> {
     }
 };
 
+// fp32 as three bf16 planes: 24 bits of mantissa are 8 + 8 + 8, so x = a + b + c exactly (down to 2^-126), with fp32's range.  A product is
+// six 16-bit matrix instructions, the terms above 2^-24 of it, in 192 cycles where eight 32-bit ones take 512.
+struct X3;
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+struct Frag3 {
+    bf16x8 p[3];
+};
+template <>
+struct Mma<X3> {
+    typedef Frag3 frag;
+    static __device__ __forceinline__ f32x16 run(const frag& a, const frag& b, f32x16 c) {
+#pragma unroll
+        for (int i = 2; i >= 0; --i)                                      // small terms first
+#pragma unroll
+            for (int j = i; j >= 0; --j) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[i - j], b.p[j], c, 0, 0, 0);
+        return c;
+    }
+};
+
 template <typename T>
 using Frag = typename Mma<T>::frag;
 
+// What tensors hold in memory, what tiles hold in LDS, planes of a tile.
+template <typename T>
+struct Type {
+    typedef T mem, elem;
+    static constexpr int PLANES = 1;
+};
+template <>
+struct Type<X3> {
+    typedef float mem;
+    typedef bf16 elem;
+    static constexpr int PLANES = 3;
+};
+template <typename T>
+using Mem = typename Type<T>::mem;
+template <typename T>
+using Elem = typename Type<T>::elem;
+
+// The planes of 8 values.  FINITE values only: infinity less infinity is no rest.
+template <bool FINITE>
+__device__ __forceinline__ Frag3 split8(const float (&x)[8]) {
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    Frag3 f;
+    float r[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = x[j];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        u32x4 w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = __builtin_amdgcn_perm(__float_as_uint(r[2 * j + 1]), __float_as_uint(r[2 * j]), 0x07060302);
+        f.p[k] = __builtin_bit_cast(bf16x8, w);
+        if (k < 2)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float rest = r[j] - __uint_as_float(__float_as_uint(r[j]) & 0xffff0000u);
+                r[j] = FINITE || fabsf(x[j]) != INFINITY ? rest : 0.f;
+            }
+    }
+    return f;
+}
+
 template <typename T>
 __device__ __forceinline__ Frag<T> zero_frag() {
-    Frag<T> f;
+    if constexpr (__is_same(T, X3)) {
+        const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        return split8<true>(z);
+    } else {
+        Frag<T> f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = (T)0.f;
-    return f;
+        for (int j = 0; j < 8; ++j) f[j] = (T)0.f;
+        return f;
+    }
 }
 
 // 8 consecutive channels from global memory
 template <typename T>
-__device__ __forceinline__ Frag<T> load8(const T* p) {
-    typedef Frag<T> at16 __attribute__((aligned(16)));
-    return *reinterpret_cast<const at16*>(p);
+__device__ __forceinline__ Frag<T> load8(const Mem<T>* p) {
+    if constexpr (__is_same(T, X3)) {
+        typedef f32x8 at16 __attribute__((aligned(16)));
+        const f32x8 v = *reinterpret_cast<const at16*>(p);
+        const float x[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
+        return split8<false>(x);
+    } else {
+        typedef Frag<T> at16 __attribute__((aligned(16)));
+        return *reinterpret_cast<const at16*>(p);
+    }
 }
 
 // How a tile of DP channels a row lies in LDS, and where this lane reads it.  Both ways of reading have to spread over all 64 banks: as A
@@ -76,15 +147,14 @@ __device__ __forceinline__ Frag<T> load8(const T* p) {
 // value over 16 rows (the other).  A lane's row is the same modulo 16 in every read, so the permutation is one exclusive or with a
 // constant.  Padded rows (272 or 288 bytes) cost the dk / dv kernel 35 % of its LDS cycles in conflicts; this order has none.
 template <typename T, int DP>
-struct Lds {
+struct LdsPlane {
     static constexpr bool HALF = sizeof(T) == 2;
     static constexpr int CH = DP * sizeof(T) / 16, E = 16 / sizeof(T);    // chunks a row, elements a chunk
-    static constexpr int TILE = KT * DP;                                  // elements of 64 rows
     int rows, cols;                                                       // this lane's offsets
     static __host__ __device__ constexpr int order(int r) {
         return CH >= 16 ? (r & 3) << 2 | (r >> 2 & 3) : CH == 8 ? (r >> 1 & 1) << 2 | (r >> 2 & 3) : r >> 2 & 3;
     }
-    __device__ __forceinline__ explicit Lds(int lane) {
+    __device__ __forceinline__ explicit LdsPlane(int lane) {
         const int i = lane & 15, half = lane >> 5, r = 4 * half + (i >> 2);
         rows = (lane & 31) * DP + ((HALF ? half : 2 * half) ^ order(lane & 31)) * E;
         cols = HALF ? r * DP + (((lane & 16) / 8 + (i >> 1 & 1)) ^ order(r)) * E + 4 * (i & 1) : 4 * half * DP + ((lane & 31) ^ order(4 * half) * E);
@@ -118,19 +188,50 @@ struct Lds {
     }
 };
 
+// Rows of a staged tile: 64, 32 where three planes of 64 channels or more would leave one workgroup a CU.
+template <typename T, int DP>
+constexpr int ROWS = __is_same(T, X3) && DP >= 64 ? 32 : 64;
+
+// The planes of a tile, one behind the other.
+template <typename T, int DP>
+struct Lds : LdsPlane<Elem<T>, DP> {
+    typedef LdsPlane<Elem<T>, DP> Plane;
+    static constexpr int PLANES = Type<T>::PLANES, PLANE = ROWS<T, DP> * DP, TILE = PLANES * PLANE;
+    using Plane::Plane;
+    __device__ __forceinline__ Frag<T> read_rows(const Elem<T>* tile, int row, int col) const {
+        if constexpr (PLANES == 1) {
+            return Plane::read_rows(tile, row, col);
+        } else {
+            return {Plane::read_rows(tile, row, col), Plane::read_rows(tile + PLANE, row, col), Plane::read_rows(tile + 2 * PLANE, row, col)};
+        }
+    }
+    __device__ __forceinline__ Frag<T> read_cols(const Elem<T>* tile, int row, int col) const {
+        if constexpr (PLANES == 1) {
+            return Plane::read_cols(tile, row, col);
+        } else {
+            return {Plane::read_cols(tile, row, col), Plane::read_cols(tile + PLANE, row, col), Plane::read_cols(tile + 2 * PLANE, row, col)};
+        }
+    }
+};
+
 // Registers 8 t .. 8 t + 7 of a score tile as the other operand (round to nearest even).
 template <typename T>
 __device__ __forceinline__ Frag<T> pack8(const f32x16& s, int t) {
-    Frag<T> f;
+    if constexpr (__is_same(T, X3)) {
+        const float x[8] = {s[8 * t], s[8 * t + 1], s[8 * t + 2], s[8 * t + 3], s[8 * t + 4], s[8 * t + 5], s[8 * t + 6], s[8 * t + 7]};
+        return split8<true>(x);
+    } else {
+        Frag<T> f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = (T)s[8 * t + j];
-    return f;
+        for (int j = 0; j < 8; ++j) f[j] = (T)s[8 * t + j];
+        return f;
+    }
 }
 
 // Waves a SIMD that the forward and dq kernels are compiled for: two (256 registers a wave), so that one wave's exponentials run beside the
 // other's products.  fp32 at D = 128 holds twice the operands and would spill.
 template <typename T, int DP>
-constexpr int WAVES = sizeof(T) == 4 && DP == 128 ? 1 : 2;
+constexpr int WAVES = sizeof(Mem<T>) == 4 && DP == 128 ? 1 : 2;
 
 struct Tensor {
     const void* p;
@@ -139,6 +240,8 @@ struct Tensor {
 
 struct Attn {
     Tensor q, k, v, dout, out;
+    Tensor qt, kt, vt, dt;                 // q, k, v, dout as tiles are fetched from: themselves, or the first of their planes
+    int64_t plane_q, plane_k;              // elements between planes
     const int* lens;
     const uint8_t* mask;                   // [N, S]
     void* o[2];                            // results (out, or dq, or dk and dv): dense, in T or, with splits, 32-bit partials
@@ -186,26 +289,32 @@ struct Job {
 
 __device__ __forceinline__ int valid_len(const Attn& a, int n) { return a.lens ? min(max(a.lens[n], 0), a.S) : a.S; }
 
-// A tile of ROWS rows x DP channels on its way from memory into LDS, by LDS-DMA: no register holds it and no vector instruction moves it.
+// A tile of NROWS rows x DP channels on its way from memory into LDS, by LDS-DMA: no register holds it and no vector instruction moves it.
 // Every thread fetches 16 bytes an instruction; the chunk order of Lds is applied to the source address.  Rows behind the last and channels
 // behind D lie outside the buffer descriptor and arrive as zeros.
-template <typename T, int DP, int ROWS, int THREADS>
+template <typename T, int DP, int NROWS, int THREADS>
 struct Dma {
-    typedef Lds<T, DP> L;
-    static constexpr int CH = L::CH, PER = ROWS * CH / THREADS, RPI = THREADS / CH;   // instructions a tile, rows an instruction
+    typedef LdsPlane<Elem<T>, DP> L;
+    static constexpr int CH = L::CH, PER = NROWS * CH / THREADS, RPI = THREADS / CH;   // instructions a plane, rows an instruction
+    static_assert(NROWS * CH % THREADS == 0, "every thread fetches the same number of chunks");
+    int64_t plane;
     unsigned off, step, row_bytes, stride;
-    __device__ __forceinline__ Dma(int64_t stride_, int D) : stride((unsigned)(stride_ * sizeof(T))) {
-        row_bytes = D * (unsigned)sizeof(T);
+    __device__ __forceinline__ Dma(int64_t stride_, int D, int64_t plane_) : plane(plane_), stride((unsigned)(stride_ * sizeof(Elem<T>))) {
+        row_bytes = D * (unsigned)sizeof(Elem<T>);
         off = threadIdx.x / CH * stride;
         step = RPI * stride;
     }
     // rows base .. base + rows - 1 (rows > 0); base, rows and tile are the same in every lane
-    __device__ __forceinline__ void issue(const T* base, int rows, T* tile) const {
+    __device__ __forceinline__ void issue(const Elem<T>* base, int rows, Elem<T>* tile) const {
+#pragma unroll
+        for (int k = 0; k < Type<T>::PLANES; ++k) issue_plane(base + k * plane, rows, tile + k * NROWS * DP);
+    }
+    __device__ __forceinline__ void issue_plane(const Elem<T>* base, int rows, Elem<T>* tile) const {
         typedef int i32x4 __attribute__((ext_vector_type(4)));
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const uint64_t at = reinterpret_cast<uint64_t>(base);
         const i32x4 rsrc = {__builtin_amdgcn_readfirstlane((int)at), __builtin_amdgcn_readfirstlane((int)(at >> 32) & 0xffff),
-                            __builtin_amdgcn_readfirstlane((int)((unsigned)(min(rows, ROWS) - 1) * stride + row_bytes)), 0x00020000};
+                            __builtin_amdgcn_readfirstlane((int)((unsigned)(min(rows, NROWS) - 1) * stride + row_bytes)), 0x00020000};
         const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) void*)tile) + wave * 1024;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
@@ -213,23 +322,23 @@ struct Dma {
             // channels behind D: an offset no descriptor reaches (strides are below 2^23 elements)
             const unsigned o = c < row_bytes ? off + step * i + c : 0xff000000u;
             // As assembly (it writes no register) because the compiler lets every LDS read wait for its own form of this load.  The waits:
-            // five states from a lane read's scalar to a memory instruction that uses it, one from m0.
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to + i * THREADS * 16), "v"(o), "s"(rsrc) : "memory", "m0");
+            // five states from a lane read's scalar to a memory instruction that uses it, one from m0 (which nothing else here uses).
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to + i * THREADS * 16), "v"(o), "s"(rsrc) : "memory");
         }
     }
 };
 
 __device__ __forceinline__ void dma_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-// Zeros over the rows whose bit in `keep` is 0, by 256 threads.
+// Zeros over the rows of a tile whose bit in `keep` is 0, by 256 threads.
 template <typename T, int DP>
-__device__ __forceinline__ void zero_rows(T* tile, unsigned long long keep) {
-    constexpr int CH = Lds<T, DP>::CH;
+__device__ __forceinline__ void zero_rows(Elem<T>* tile, unsigned long long keep) {
+    typedef Lds<T, DP> L;
     unsigned e = threadIdx.x;
     asm volatile("" : "+v"(e));            // keeps this branch's addresses out of the loop's registers
 #pragma unroll
-    for (int i = 0; i < KT * CH / 256; ++i, e += 256)
-        if (!(keep >> (e / CH) & 1)) *reinterpret_cast<f32x4*>(tile + e * Lds<T, DP>::E) = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < L::TILE / L::E / 256; ++i, e += 256)
+        if (!(keep >> (e / L::CH % ROWS<T, DP>) & 1)) *reinterpret_cast<f32x4*>(tile + e * L::E) = f32x4{0.f, 0.f, 0.f, 0.f};
 }
 
 // The mask byte of key s0 + lane, one tile ahead of its use; 1 without a mask.
@@ -237,10 +346,14 @@ __device__ __forceinline__ unsigned key_mask(const Attn& a, int n, int s0) {
     return a.mask ? a.mask[(int64_t)n * a.S + min(s0 + (int)(threadIdx.x & 63), a.S - 1)] : 1u;
 }
 
-// Bits of the keys s0 .. s0 + 63 that are there; the same in every wave.
+// Bits of the KT keys from s0 on that are there; the same in every wave.
+template <int KT>
 __device__ __forceinline__ unsigned long long key_bits(unsigned mask, int s0, int end) {
-    return __ballot(s0 + (int)(threadIdx.x & 63) < end && mask != 0);
+    const int i = threadIdx.x & 63;
+    return __ballot(i < KT && s0 + i < end && mask != 0);
 }
+template <int KT>
+constexpr unsigned long long ALL_KEYS = KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1;
 
 // Scores of keys that are not there become -inf, whatever they were: bits of 32 keys, this lane's half shifted to bit 0.
 __device__ __forceinline__ void drop_keys(f32x16& st, unsigned bits) {
@@ -300,7 +413,7 @@ struct ColumnScale {
     float f = 1.f, seen = 0.f;
     template <int NB>
     __device__ __forceinline__ void apply(f32x16 (&ds)[NB], f32x16 (&acc)[DB]) {
-        if constexpr (sizeof(T) == 2 && !__is_same(T, bf16)) {
+        if constexpr (__is_same(T, f16)) {
             float m = 0.f;
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -333,10 +446,10 @@ struct ColumnScale {
 // 4 waves x 32 rows a workgroup; tiles of 64 keys, two in LDS.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_forward_kernel(const Attn a) {
-    constexpr int DB = DP / 32, KS = DP / 16, TILE = Lds<T, DP>::TILE;
+    constexpr int DB = DP / 32, KS = DP / 16, TILE = Lds<T, DP>::TILE, KT = ROWS<T, DP>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    T* ks = reinterpret_cast<T*>(smem);
-    T* vs = ks + 2 * TILE;
+    Elem<T>* ks = reinterpret_cast<Elem<T>*>(smem);
+    Elem<T>* vs = ks + 2 * TILE;
     const Job job(a);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Lds<T, DP> lds(lane);
@@ -347,19 +460,19 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_forward_kernel(const
     const int beg = min(len, job.split * per), end = min(len, beg + per);
 
     Frag<T> qf[KS];
-    const T* qp = static_cast<const T*>(a.q.p) + job.n * a.q.n + (int64_t)min(l, a.L - 1) * a.q.l + h * a.q.h;
+    const Mem<T>* qp = static_cast<const Mem<T>*>(a.q.p) + job.n * a.q.n + (int64_t)min(l, a.L - 1) * a.q.l + h * a.q.h;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
         const int c = 16 * s + 8 * (lane >> 5);
         qf[s] = r < R && c < a.D ? load8<T>(qp + c) : zero_frag<T>();
     }
-    const T* kb = static_cast<const T*>(a.k.p) + job.n * a.k.n + job.hk * a.k.h;
-    const T* vb = static_cast<const T*>(a.v.p) + job.n * a.v.n + job.hk * a.v.h;
-    const Dma<T, DP, KT, 256> dk(a.k.l, a.D), dv(a.v.l, a.D);
+    const Elem<T>* kb = static_cast<const Elem<T>*>(a.kt.p) + job.n * a.kt.n + job.hk * a.kt.h;
+    const Elem<T>* vb = static_cast<const Elem<T>*>(a.vt.p) + job.n * a.vt.n + job.hk * a.vt.h;
+    const Dma<T, DP, KT, 256> dk(a.kt.l, a.D, a.plane_k), dv(a.vt.l, a.D, a.plane_k);
     unsigned mask = 0;
     auto fetch = [&](int s0, int buf) {
-        dk.issue(kb + s0 * a.k.l, end - s0, ks + buf * TILE);
-        dv.issue(vb + s0 * a.v.l, end - s0, vs + buf * TILE);
+        dk.issue(kb + s0 * a.kt.l, end - s0, ks + buf * TILE);
+        dv.issue(vb + s0 * a.vt.l, end - s0, vs + buf * TILE);
         mask = key_mask(a, job.n, s0);
     };
     f32x16 acc[DB];
@@ -370,32 +483,31 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_forward_kernel(const
     if (beg < end) fetch(beg, 0);
     int buf = 0;
     for (int s0 = beg; s0 < end; s0 += KT, buf ^= 1) {
-        const T* kt = ks + buf * TILE;
-        T* vt = vs + buf * TILE;
+        const Elem<T>* kt = ks + buf * TILE;
+        Elem<T>* vt = vs + buf * TILE;
         dma_landed();
-        const unsigned long long bits = key_bits(mask, s0, end);
+        const unsigned long long bits = key_bits<KT>(mask, s0, end);
         __syncthreads();                    // all of the tile is there, and the other buffer's readers are done
-        if (a.mask && ~bits && bits) {      // a weight of 0 does not undo a NaN in v
+        if (a.mask && bits != ALL_KEYS<KT> && bits) {      // a weight of 0 does not undo a NaN in v
             zero_rows<T, DP>(vt, bits);
             __syncthreads();
         }
         if (s0 + KT < end) fetch(s0 + KT, buf ^ 1);
         if (bits == 0) continue;
-        f32x16 st[2];
+        f32x16 st[KT / 32];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < KT / 32; ++b) {
             st[b] = splat16(0.f);
 #pragma unroll
             for (int s = 0; s < KS; ++s) st[b] = Mma<T>::run(lds.read_rows(kt, 32 * b, 16 * s), qf[s], st[b]);
         }
-        if (~bits) {
-            const unsigned long long mine = bits >> 4 * (lane >> 5);
-            drop_keys(st[0], (unsigned)mine);
-            drop_keys(st[1], (unsigned)(mine >> 32));
+        if (bits != ALL_KEYS<KT>) {
+#pragma unroll
+            for (int b = 0; b < KT / 32; ++b) drop_keys(st[b], (unsigned)(bits >> 32 * b >> 4 * (lane >> 5)));
         }
         float t = NEG;
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < KT / 32; ++b)
 #pragma unroll
             for (int j = 0; j < 16; ++j) t = fmaxf(t, st[b][j]);
         t = fmaxf(t, dfsfm::from_xor32(t, lane)) * c;
@@ -411,7 +523,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_forward_kernel(const
         }
         const float mm = m == NEG ? 0.f : m;
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < KT / 32; ++b) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
                 st[b][j] = __builtin_amdgcn_exp2f(fmaf(st[b][j], c, -mm));
@@ -436,14 +548,16 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_forward_kernel(const
             ml[1] = sum;
         }
     } else {
-        store_col<T, DB, true>(static_cast<T*>(a.o[0]) + row * a.D, acc, sum > 0.f || sum != sum ? 1.f / sum : 0.f, a.D, lane);
+        store_col<Mem<T>, DB, true>(static_cast<Mem<T>*>(a.o[0]) + row * a.D, acc, sum > 0.f || sum != sum ? 1.f / sum : 0.f, a.D, lane);
         if (lane < 32) a.lse[at] = fmaf(m == NEG ? 0.f : m, LN2, logf(sum));
     }
 }
 
-// Joins the forward partials: 8 lanes x 4 channels a step, a row each 8 lanes.
+// Joins up to FEW_SPLITS forward partials: 8 lanes a row, 4 channels a step, the splits one after the other (76800 rows x 3 splits x 32:
+// 12 us, 39 with a wave a row; 128 rows x 14 x 64: 13 us against 4.7).
+constexpr int FEW_SPLITS = 8;
 template <typename T>
-__global__ __launch_bounds__(256) void attn_join_kernel(const Attn a) {
+__global__ __launch_bounds__(256) void attn_join_few_kernel(const Attn a) {
     const int64_t rows = (int64_t)a.N * a.L * a.H, row = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
     if (row >= rows) return;
     const int h = (int)(row % a.H);
@@ -467,6 +581,58 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const Attn a) {
         dfsfm::store_f32<T, 4>(static_cast<T*>(a.o[1]) + row * a.D + d, 4, o);
     }
     if ((threadIdx.x & 7) == 0) a.lse[at] = fmaf(mm, LN2, logf(sum));
+}
+
+// Joins more of them, a wave a row: the lanes share the splits' maxima and sums, then 4 channels and every SG-th split each.
+constexpr int MAX_SPLITS = 256;
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_kernel(const Attn a) {
+    __shared__ float weight[4][MAX_SPLITS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t rows = (int64_t)a.N * a.L * a.H, row = (int64_t)blockIdx.x * 4 + wave, at0 = min(row, rows - 1);
+    const int h = (int)(at0 % a.H);
+    const int64_t nl = at0 / a.H, at = (nl / a.L * a.H + h) * a.L + nl % a.L;
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const f32x2* ml = reinterpret_cast<const f32x2*>(a.ml) + at;
+    f32x2 v[MAX_SPLITS / 64];
+    float m = NEG, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < MAX_SPLITS / 64; ++i) {
+        const int s = lane + 64 * i;
+        v[i] = s < a.splits ? ml[s * rows] : f32x2{NEG, 0.f};
+        m = fmaxf(m, v[i][0]);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    const float mm = m == NEG ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < MAX_SPLITS / 64; ++i) {
+        v[i][0] = __builtin_amdgcn_exp2f(v[i][0] - mm);
+        sum = fmaf(v[i][1], v[i][0], sum);
+        weight[wave][lane + 64 * i] = v[i][0];
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
+    __syncthreads();
+    if (row >= rows) return;
+    const int lanes = a.D <= 32 ? 8 : a.D <= 64 ? 16 : 32, d = lane % lanes * 4;
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+    if (d < a.D)
+#pragma unroll 4
+        for (int s = lane / lanes; s < a.splits; s += 64 / lanes) {
+            const float f = weight[wave][s];
+            const f32x4 t = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.o[0]) + s * a.numel + row * a.D + d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(t[e], f, o[e]);
+        }
+    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    for (int x = lanes; x < 64; x <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], x);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = within_range<T>(o[e] * inv);
+    if (d < a.D && lane < lanes) dfsfm::store_f32<T, 4>(static_cast<T*>(a.o[1]) + row * a.D + d, 4, o);
+    if (lane == 0) a.lse[at] = fmaf(mm, LN2, logf(sum));
 }
 
 // ---------------------------------------------------------------- backward
@@ -500,10 +666,10 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(const Attn a) {
 // costs).  Two of three products are then made twice, over two tiles at most; a pass over dout and out is saved.
 template <typename T, int DP, bool SHORT>
 __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn a) {
-    constexpr int DB = DP / 32, KS = DP / 16, TILE = Lds<T, DP>::TILE;
+    constexpr int DB = DP / 32, KS = DP / 16, TILE = Lds<T, DP>::TILE, KT = ROWS<T, DP>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    T* ks = reinterpret_cast<T*>(smem);
-    T* vs = ks + 2 * TILE;
+    Elem<T>* ks = reinterpret_cast<Elem<T>*>(smem);
+    Elem<T>* vs = ks + 2 * TILE;
     const Job job(a);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Lds<T, DP> lds(lane);
@@ -514,8 +680,8 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
     const int beg = min(len, job.split * per), end = min(len, beg + per);
 
     Frag<T> qf[KS], of[KS];
-    const T* qp = static_cast<const T*>(a.q.p) + job.n * a.q.n + (int64_t)min(l, a.L - 1) * a.q.l + h * a.q.h;
-    const T* op = static_cast<const T*>(a.dout.p) + job.n * a.dout.n + (int64_t)min(l, a.L - 1) * a.dout.l + h * a.dout.h;
+    const Mem<T>* qp = static_cast<const Mem<T>*>(a.q.p) + job.n * a.q.n + (int64_t)min(l, a.L - 1) * a.q.l + h * a.q.h;
+    const Mem<T>* op = static_cast<const Mem<T>*>(a.dout.p) + job.n * a.dout.n + (int64_t)min(l, a.L - 1) * a.dout.l + h * a.dout.h;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
         const int c = 16 * s + 8 * (lane >> 5);
@@ -526,18 +692,18 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
     const float c = a.scale * LOG2E, lse = r < R ? a.lse[at] : NEG;
     const float lse2 = lse == NEG ? INFINITY : lse * LOG2E;              // a row without keys has p = 0
     float delta = !SHORT && r < R ? a.delta[at] : 0.f;
-    const T* kb = static_cast<const T*>(a.k.p) + job.n * a.k.n + job.hk * a.k.h;
-    const T* vb = static_cast<const T*>(a.v.p) + job.n * a.v.n + job.hk * a.v.h;
-    const Dma<T, DP, KT, 256> dk(a.k.l, a.D), dv(a.v.l, a.D);
+    const Elem<T>* kb = static_cast<const Elem<T>*>(a.kt.p) + job.n * a.kt.n + job.hk * a.kt.h;
+    const Elem<T>* vb = static_cast<const Elem<T>*>(a.vt.p) + job.n * a.vt.n + job.hk * a.vt.h;
+    const Dma<T, DP, KT, 256> dk(a.kt.l, a.D, a.plane_k), dv(a.vt.l, a.D, a.plane_k);
     unsigned mask = 0;
     auto fetch = [&](int s0, int buf) {
-        dk.issue(kb + s0 * a.k.l, end - s0, ks + buf * TILE);
-        dv.issue(vb + s0 * a.v.l, end - s0, vs + buf * TILE);
+        dk.issue(kb + s0 * a.kt.l, end - s0, ks + buf * TILE);
+        dv.issue(vb + s0 * a.vt.l, end - s0, vs + buf * TILE);
         mask = key_mask(a, job.n, s0);
     };
     // keys that the mask drops: p is 0, which does not undo a NaN in dp or k
     auto clear = [&](int buf, unsigned long long bits) {
-        if (a.mask && ~bits && bits) {
+        if (a.mask && bits != ALL_KEYS<KT> && bits) {
             zero_rows<T, DP>(ks + buf * TILE, bits);
             zero_rows<T, DP>(vs + buf * TILE, bits);
             __syncthreads();
@@ -549,8 +715,8 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
     ColumnScale<T, DB> cs;
     // p dp of 32 keys, dp less delta
     auto products = [&](int buf, int b, unsigned long long bits, f32x16& ds) {
-        const T* kt = ks + buf * TILE;
-        const T* vt = vs + buf * TILE;
+        const Elem<T>* kt = ks + buf * TILE;
+        const Elem<T>* vt = vs + buf * TILE;
         f32x16 st = splat16(0.f);
         ds = splat16(-delta);
 #pragma unroll
@@ -558,13 +724,13 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
             st = Mma<T>::run(lds.read_rows(kt, 32 * b, 16 * s), qf[s], st);
             ds = Mma<T>::run(lds.read_rows(vt, 32 * b, 16 * s), of[s], ds);
         }
-        if (~bits) drop_keys(st, (unsigned)(bits >> 32 * b >> 4 * (lane >> 5)));
+        if (bits != ALL_KEYS<KT>) drop_keys(st, (unsigned)(bits >> 32 * b >> 4 * (lane >> 5)));
 #pragma unroll
         for (int j = 0; j < 16; ++j) ds[j] *= __builtin_amdgcn_exp2f(fmaf(st[j], c, -lse2));
     };
     auto accumulate = [&](int buf, unsigned long long bits) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < KT / 32; ++b) {
             f32x16 ds[1];
             products(buf, b, bits, ds[0]);
             cs.apply(ds, acc);
@@ -588,14 +754,14 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
             }
         dma_landed();
 #pragma unroll
-        for (int t = 0; t < 2; ++t) bits[t] = key_bits(masks[t], t * KT, end);
+        for (int t = 0; t < 2; ++t) bits[t] = key_bits<KT>(masks[t], t * KT, end);
         __syncthreads();
         clear(0, bits[0]);
         clear(1, bits[1]);
         float sum = 0.f;
         for (int t = 0; t * KT < end; ++t)
             if (bits[t]) {
-                for (int b = 0; b < 2; ++b) {
+                for (int b = 0; b < KT / 32; ++b) {
                     f32x16 ds;
                     products(t, b, bits[t], ds);
 #pragma unroll
@@ -611,7 +777,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
         int buf = 0;
         for (int s0 = beg; s0 < end; s0 += KT, buf ^= 1) {
             dma_landed();
-            const unsigned long long bits = key_bits(mask, s0, end);
+            const unsigned long long bits = key_bits<KT>(mask, s0, end);
             __syncthreads();
             clear(buf, bits);
             if (s0 + KT < end) fetch(s0 + KT, buf ^ 1);
@@ -624,7 +790,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
     if (a.splits > 1)
         store_col<float, DB>(static_cast<float*>(a.o[0]) + job.split * a.numel + row * a.D, acc, f, a.D, lane);
     else
-        store_col<T, DB>(static_cast<T*>(a.o[0]) + row * a.D, acc, f, a.D, lane);
+        store_col<Mem<T>, DB>(static_cast<Mem<T>*>(a.o[0]) + row * a.D, acc, f, a.D, lane);
 }
 
 // dk and dv: NW waves x 32 keys a workgroup, tiles of 64 rows of q and dout, both read both ways.
@@ -634,19 +800,20 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
 // 4 x 4800 x 6400 (ragged) x 16 heads bf16 takes 1.21 - 1.31 ms; with V in registers, four waves and one wave a SIMD 2.3; with the two halves
 // of the work on two waves that pass p through LDS 1.7; as two launches, one product made twice, 1.8.
 template <typename T, int DP>
-constexpr int KEY_WAVES = DP == 128 && sizeof(T) == 2 ? 8 : 4;
+constexpr int KEY_WAVES = DP == 128 && sizeof(Mem<T>) == 2 ? 8 : 4;
 
 template <typename T, int DP>
 __global__ __launch_bounds__((64 * KEY_WAVES<T, DP>), (KEY_WAVES<T, DP> / 4)) void attn_dkdv_kernel(const Attn a) {
     constexpr int NW = KEY_WAVES<T, DP>, THREADS = 64 * NW;
     constexpr bool VLDS = NW == 8;
-    constexpr int DB = DP / 32, KS = DP / 16, TILE = Lds<T, DP>::TILE;
+    constexpr int UNROLL = VLDS ? 1 : 2;
+    constexpr int DB = DP / 32, KS = DP / 16, TILE = Lds<T, DP>::TILE, KT = ROWS<T, DP>;
     // p of fp16 tensors times 2^14: a power of two that keeps weights down to 2^-28 exact and 1 in range
     constexpr float SHIFT = __is_same(T, f16) ? 14.f : 0.f, UNSHIFT = __is_same(T, f16) ? 1.f / 16384.f : 1.f;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    T* qs = reinterpret_cast<T*>(smem);
-    T* os = qs + 2 * TILE;
-    T* vs = os + 2 * TILE;                                                // VLDS: the workgroup's keys
+    Elem<T>* qs = reinterpret_cast<Elem<T>*>(smem);
+    Elem<T>* os = qs + 2 * TILE;
+    Elem<T>* vs = os + 2 * TILE;                                                // VLDS: the workgroup's keys
     float* rowv = reinterpret_cast<float*>(vs + (VLDS ? NW * 32 * DP : 0));      // [2][2][64]: -lse / scale, -delta
     const Job job(a, NW * 32);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hkv = a.H / a.G;
@@ -660,29 +827,29 @@ __global__ __launch_bounds__((64 * KEY_WAVES<T, DP>), (KEY_WAVES<T, DP> / 4)) vo
     const int beg = min(lt * a.G, job.split * per), end = min(lt * a.G, beg + per);
 
     Frag<T> kf[KS], vf[VLDS ? 1 : KS];
-    const T* kp = static_cast<const T*>(a.k.p) + job.n * a.k.n + (int64_t)min(s, a.S - 1) * a.k.l + job.hk * a.k.h;
-    const T* vp = static_cast<const T*>(a.v.p) + job.n * a.v.n + (int64_t)min(s, a.S - 1) * a.v.l + job.hk * a.v.h;
+    const Mem<T>* kp = static_cast<const Mem<T>*>(a.k.p) + job.n * a.k.n + (int64_t)min(s, a.S - 1) * a.k.l + job.hk * a.k.h;
+    const Mem<T>* vp = static_cast<const Mem<T>*>(a.v.p) + job.n * a.v.n + (int64_t)min(s, a.S - 1) * a.v.l + job.hk * a.v.h;
 #pragma unroll
     for (int x = 0; x < KS; ++x) {
         const int c = 16 * x + 8 * (lane >> 5);
         kf[x] = there && c < a.D ? load8<T>(kp + c) : zero_frag<T>();
         if constexpr (!VLDS) vf[x] = there && c < a.D ? load8<T>(vp + c) : zero_frag<T>();
     }
-    const T* qb = static_cast<const T*>(a.q.p) + job.n * a.q.n + job.hk * a.G * a.q.h;
-    const T* ob = static_cast<const T*>(a.dout.p) + job.n * a.dout.n + job.hk * a.G * a.dout.h;
+    const Elem<T>* qb = static_cast<const Elem<T>*>(a.qt.p) + job.n * a.qt.n + job.hk * a.G * a.qt.h;
+    const Elem<T>* ob = static_cast<const Elem<T>*>(a.dt.p) + job.n * a.dt.n + job.hk * a.G * a.dt.h;
     const int64_t vec = ((int64_t)job.n * a.H + job.hk * a.G) * a.L;
-    const Dma<T, DP, KT, THREADS> dq(a.q.l, a.D), dd(a.dout.l, a.D);
-    float rv = 0.f;                         // threads 0..63: lse of a row, 64..127: delta
+    const Dma<T, DP, KT, THREADS> dq(a.qt.l, a.D, a.plane_q), dd(a.dt.l, a.D, a.plane_q);
+    float rv = 0.f;                         // threads below KT: lse of a row, the next KT: delta
     const float inv_scale = 1.f / a.scale;
     int rows = 0;                           // rows of the tile in flight
     auto fetch = [&](int it, int buf) {
         const int g = it / lt, l0 = (it - g * lt) * KT;
         rows = a.L - l0;
-        dq.issue(qb + g * a.q.h + l0 * a.q.l, rows, qs + buf * TILE);
-        dd.issue(ob + g * a.dout.h + l0 * a.dout.l, rows, os + buf * TILE);
-        if (threadIdx.x < 128) {
-            const int row = threadIdx.x & 63;
-            rv = (threadIdx.x < 64 ? a.lse : a.delta)[vec + (int64_t)g * a.L + l0 + min(row, rows - 1)];
+        dq.issue(qb + g * a.qt.h + l0 * a.qt.l, rows, qs + buf * TILE);
+        dd.issue(ob + g * a.dt.h + l0 * a.dt.l, rows, os + buf * TILE);
+        if (threadIdx.x < 2 * KT) {
+            const int row = threadIdx.x % KT;
+            rv = (threadIdx.x < KT ? a.lse : a.delta)[vec + (int64_t)g * a.L + l0 + min(row, rows - 1)];
         }
     };
     f32x16 dk[DB], dv[DB];
@@ -694,31 +861,31 @@ __global__ __launch_bounds__((64 * KEY_WAVES<T, DP>), (KEY_WAVES<T, DP> / 4)) vo
     if (any && beg < end) {
         if constexpr (VLDS) {               // masked keys come as they are: a key's column is its own, and dropped at the end
             const int s0 = job.tile * (NW * 32);
-            const Dma<T, DP, NW * 32, THREADS> dv(a.v.l, a.D);
-            dv.issue(static_cast<const T*>(a.v.p) + job.n * a.v.n + job.hk * a.v.h + s0 * a.v.l, len - s0, vs);
+            const Dma<T, DP, NW * 32, THREADS> dv(a.vt.l, a.D, a.plane_k);
+            dv.issue(static_cast<const Elem<T>*>(a.vt.p) + job.n * a.vt.n + job.hk * a.vt.h + s0 * a.vt.l, len - s0, vs);
         }
         fetch(beg, 0);
     }
     const bool mine = __ballot(there) != 0;
     int buf = 0;
     for (int it = beg; any && it < end; ++it, buf ^= 1) {
-        T* qt = qs + buf * TILE;
-        T* ot = os + buf * TILE;
-        float* vt = rowv + buf * 128;
+        const Elem<T>* qt = qs + buf * TILE;
+        const Elem<T>* ot = os + buf * TILE;
+        float* vt = rowv + buf * 2 * KT;
         dma_landed();
         // -lse / scale and -delta start the sums; a row without keys, or behind the last, gets a score of -inf: p = 0
-        if (threadIdx.x < 128) {
-            const bool in = (int)(threadIdx.x & 63) < rows;
-            vt[threadIdx.x] = threadIdx.x < 64 ? (in && rv != NEG ? -rv * inv_scale : NEG) : (in ? -rv : 0.f);
+        if (threadIdx.x < 2 * KT) {
+            const bool in = (int)(threadIdx.x % KT) < rows;
+            vt[threadIdx.x] = threadIdx.x < KT ? (in && rv != NEG ? -rv * inv_scale : NEG) : (in ? -rv : 0.f);
         }
         __syncthreads();
         if (it + 1 < end) fetch(it + 1, buf ^ 1);
         if (!mine) continue;
-#pragma unroll(VLDS ? 1 : 2)
-        for (int b = 0; b < 2; ++b) {
+#pragma unroll UNROLL
+        for (int b = 0; b < KT / 32; ++b) {
             f32x16 st = rows16(vt + 32 * b, lane);
             f32x16 ds[1];
-            ds[0] = rows16(vt + 64 + 32 * b, lane);
+            ds[0] = rows16(vt + KT + 32 * b, lane);
 #pragma unroll
             for (int x = 0; x < KS; ++x) {
                 st = Mma<T>::run(lds.read_rows(qt, 32 * b, 16 * x), kf[x], st);
@@ -753,8 +920,8 @@ __global__ __launch_bounds__((64 * KEY_WAVES<T, DP>), (KEY_WAVES<T, DP> / 4)) vo
         store_col<float, DB>(static_cast<float*>(a.o[0]) + job.split * a.numel + row * a.D, dk, f, a.D, lane);
         store_col<float, DB>(static_cast<float*>(a.o[1]) + job.split * a.numel + row * a.D, dv, UNSHIFT, a.D, lane);
     } else {
-        store_col<T, DB>(static_cast<T*>(a.o[0]) + row * a.D, dk, f, a.D, lane);
-        store_col<T, DB>(static_cast<T*>(a.o[1]) + row * a.D, dv, UNSHIFT, a.D, lane);
+        store_col<Mem<T>, DB>(static_cast<Mem<T>*>(a.o[0]) + row * a.D, dk, f, a.D, lane);
+        store_col<Mem<T>, DB>(static_cast<Mem<T>*>(a.o[1]) + row * a.D, dv, UNSHIFT, a.D, lane);
     }
 }
 
@@ -764,6 +931,7 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(const float* __restrict__
     const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;      // D is a multiple of 8, so numel is
     if (e >= numel) return;
     float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (int s = 0; s < splits; ++s) {
         float t[4];
         dfsfm::load_f32<float, 4>(part + s * numel + e, t);
@@ -771,6 +939,18 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(const float* __restrict__
         for (int i = 0; i < 4; ++i) o[i] += t[i];
     }
     dfsfm::store_f32<T, 4>(out + e, 4, o);
+}
+
+// The three planes of x (blockIdx.y 0) or y (1), [N, len, heads, D] fp32, dense: 8 channels a thread.
+__global__ __launch_bounds__(256) void attn_planes_kernel(const Tensor x, const Tensor y, int len, int heads, int D, bf16* __restrict__ to, int64_t plane) {
+    const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+    if (e >= plane) return;
+    const Tensor& t = blockIdx.y ? y : x;
+    const int64_t row = e / D, nl = row / heads;
+    const Frag3 f = load8<X3>(static_cast<const float*>(t.p) + nl / len * t.n + nl % len * t.l + row % heads * t.h + e % D);
+    bf16* o = to + (blockIdx.y ? 3 * plane : 0) + e;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) *reinterpret_cast<bf16x8*>(o + k * plane) = f.p[k];
 }
 
 // ---------------------------------------------------------------- host
@@ -787,7 +967,7 @@ bool rows_ok(const void* p, int64_t n, int64_t l, int64_t h, int D, int dtype) {
 // workgroups of the forward pass 2 x 4800 x 10816 x 8 x 32 fp32 take 1.21 ms, three splits of each 0.98 with the join.
 int choose_splits(int64_t groups, int64_t length, int slots) {
     if (groups <= 0 || groups >= 8 * slots) return 1;
-    const int64_t most = length / 256 < 256 ? length / 256 : 256;
+    const int64_t most = length / 256 < MAX_SPLITS ? length / 256 : MAX_SPLITS;
     int best = 1;
     double fill = 0;
     for (int s = 1; s <= most || s == 1; ++s) {
@@ -799,30 +979,59 @@ int choose_splits(int64_t groups, int64_t length, int slots) {
     return best;
 }
 
+// The launches of a call, from its sizes alone.
 struct Plan {
     int heads, tq, tk, fwd, dq, dkdv;       // row tiles, key tiles, splits
+    bool xq, xk;                            // fp32 in three planes: the kernels that walk the keys, the one that walks the rows
+    int64_t rows, keys;                     // elements of q (or out), of k
     Plan(int N, int L, int S, int H, int Hkv, int D, int dtype) {
         heads = N * Hkv;
         const int64_t R = (int64_t)L * (H / Hkv);
-        const int dp = pad_dim(D), keys = 32 * (dtype == DFSFM_F32 ? KEY_WAVES<float, 128> : dp == 128 ? KEY_WAVES<bf16, 128> : KEY_WAVES<bf16, 32>);
+        // Splitting k and v (or q and dout) costs 20 bytes an element and pays from 64 rows (or keys) a head on; fewer are bound by memory.
+        xq = dtype == DFSFM_F32 && R > 64;
+        xk = dtype == DFSFM_F32 && S > 64;
+        const int wave_keys = 32 * (dtype != DFSFM_F32 && pad_dim(D) == 128 ? KEY_WAVES<bf16, 128> : KEY_WAVES<bf16, 32>);
         tq = (int)((R + 127) / 128);
-        tk = (S + keys - 1) / keys;
-        fwd = dq = choose_splits((int64_t)heads * tq, S, 512);
-        dkdv = choose_splits((int64_t)heads * tk, R, keys == 256 ? 256 : 512);
+        tk = (S + wave_keys - 1) / wave_keys;
+        // One row tile a head reads its keys once, from memory: 2048 workgroups keep more loads under way, and a long sequence among short ones
+        // ends sooner (16 single tokens x 10816 ragged keys x 8 x 64 fp16: 4 splits 59 us, 14 splits 42, the rate of a large copy).
+        fwd = dq = choose_splits((int64_t)heads * tq, S, tq == 1 ? 2048 : 512);
+        dkdv = choose_splits((int64_t)heads * tk, R, wave_keys == 256 ? 256 : 512);
+        rows = (int64_t)N * L * H * D;
+        keys = (int64_t)N * S * Hkv * D;
+    }
+    // bytes of workspaces
+    size_t planes_k() const { return xq ? (size_t)keys * 12 : 0; }
+    size_t planes_q() const { return xk ? (size_t)rows * 12 : 0; }
+    size_t forward(int D) const { return planes_k() + (fwd > 1 ? (size_t)fwd * (rows + rows / D * 2) * 4 : 0); }
+    size_t delta(int D) const { return ((size_t)(rows / D) * 4 + 15) / 16 * 16; }
+    size_t backward(int D) const {
+        const size_t a = planes_k() + (dq > 1 ? (size_t)dq * rows * 4 : 0), b = planes_q() + (dkdv > 1 ? (size_t)2 * dkdv * keys * 4 : 0);
+        return delta(D) + (a > b ? a : b);
     }
 };
 
 bool shape_ok(int N, int L, int S, int H, int Hkv, int D) {
-    if (D <= 0 || D > 128 || D % 8 || Hkv <= 0 || H % Hkv) return false;
+    if (D <= 0 || D > 128 || D % 8 || Hkv <= 0 || H % Hkv || (int64_t)H * D >= (1 << 23)) return false;
     const int64_t R = (int64_t)L * (H / Hkv), heads = (int64_t)N * Hkv;
     // row and workgroup numbers are 32-bit
-    return R < (1ll << 30) && S < (1 << 30) && heads < (1 << 20) && heads * ((R + 127) / 128 + 512) < (1ll << 31) &&
-           heads * (((int64_t)S + 127) / 128 + 512) < (1ll << 31);
+    return R < (1ll << 30) && S < (1 << 30) && heads < (1 << 20) && heads * ((R + 127) / 128 + 2048) < (1ll << 31) &&
+           heads * (((int64_t)S + 127) / 128 + 2048) < (1ll << 31);
+}
+
+// The planes of two tensors of the same sizes, dense, at `to`; the tensors as tiles are fetched from them.
+void make_planes(const Tensor& x, const Tensor& y, int N, int len, int heads, int D, void* to, Tensor& xt, Tensor& yt, int64_t& plane, hipStream_t st) {
+    plane = (int64_t)N * len * heads * D;
+    bf16* p = static_cast<bf16*>(to);
+    xt = {p, (int64_t)len * heads * D, (int64_t)heads * D, D};
+    yt = {p + 3 * plane, (int64_t)len * heads * D, (int64_t)heads * D, D};
+    if (plane > 0)
+        hipLaunchKernelGGL(attn_planes_kernel, dim3((unsigned)((plane / 8 + 255) / 256), 2), dim3(256), 0, st, x, y, len, heads, D, p, plane);
 }
 
 template <typename T, int DP>
-int forward_dp(Attn a, const Plan& p, T* out, hipStream_t st) {
-    constexpr int smem = 4 * Lds<T, DP>::TILE * sizeof(T);
+int forward_dp(Attn a, const Plan& p, void* out, hipStream_t st) {
+    constexpr int smem = 4 * Lds<T, DP>::TILE * sizeof(Elem<T>);
     static dfsfm::SmemAttr attr;
     attr.ensure(reinterpret_cast<const void*>(&attn_forward_kernel<T, DP>), smem);
     a.tiles = p.tq;
@@ -832,75 +1041,89 @@ int forward_dp(Attn a, const Plan& p, T* out, hipStream_t st) {
     if (p.fwd > 1) {
         a.o[1] = out;
         const int64_t rows = (int64_t)a.N * a.L * a.H;
-        hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)((rows + 31) / 32)), dim3(256), 0, st, a);
+        if (p.fwd <= FEW_SPLITS)
+            hipLaunchKernelGGL((attn_join_few_kernel<Mem<T>>), dim3((unsigned)((rows + 31) / 32)), dim3(256), 0, st, a);
+        else
+            hipLaunchKernelGGL((attn_join_kernel<Mem<T>>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
     }
     return check_launch("dfsfm_cross_attention");
 }
 
 template <typename T, int DP>
-int backward_dp(Attn a, const Plan& p, T* dq, T* dk, T* dv, float* part, hipStream_t st) {
-    const int64_t rows = (int64_t)a.N * a.L * a.H, nq = rows * a.D, nk = (int64_t)a.N * a.S * (a.H / a.G) * a.D;
-    if (rows > 0) {
-        constexpr int smem = 4 * Lds<T, DP>::TILE * sizeof(T);
-        const bool few = a.S <= 2 * KT;        // one split: choose_splits cuts from 256 keys up
-        a.tiles = p.tq;
-        a.splits = p.dq;
-        a.numel = nq;
-        a.o[0] = p.dq > 1 ? static_cast<void*>(part) : dq;
-        const dim3 grid((unsigned)(p.heads * p.tq * p.dq));
-        if (few) {
-            static dfsfm::SmemAttr attr;
-            attr.ensure(reinterpret_cast<const void*>(&attn_dq_kernel<T, DP, true>), smem);
-            hipLaunchKernelGGL((attn_dq_kernel<T, DP, true>), grid, dim3(256), smem, st, a);
-        } else {
-            static dfsfm::SmemAttr attr;
-            attr.ensure(reinterpret_cast<const void*>(&attn_dq_kernel<T, DP, false>), smem);
-            hipLaunchKernelGGL((attn_delta_kernel<T>), dim3((unsigned)((rows + 31) / 32)), dim3(256), 0, st, a);
-            hipLaunchKernelGGL((attn_dq_kernel<T, DP, false>), grid, dim3(256), smem, st, a);
-        }
-        if (p.dq > 1)
-            hipLaunchKernelGGL((attn_sum_kernel<T>), dim3((unsigned)((nq / 4 + 255) / 256)), dim3(256), 0, st, part, nq, p.dq, dq);
-    }
-    if (nk > 0) {
-        a.tiles = p.tk;
-        a.splits = p.dkdv;
-        a.numel = nk;
-        a.o[0] = p.dkdv > 1 ? static_cast<void*>(part) : dk;
-        a.o[1] = p.dkdv > 1 ? static_cast<void*>(part + p.dkdv * nk) : dv;
-        constexpr int NW = KEY_WAVES<T, DP>;
-        constexpr int smem = (4 * Lds<T, DP>::TILE + (NW == 8 ? NW * 32 * DP : 0)) * sizeof(T) + 4 * KT * 4;
+int dq_dp(Attn a, const Plan& p, Mem<T>* dq, float* part, hipStream_t st) {
+    typedef Mem<T> M;
+    const int64_t rows = p.rows / a.D;
+    constexpr int smem = 4 * Lds<T, DP>::TILE * sizeof(Elem<T>);
+    const bool few = a.S <= 2 * ROWS<T, DP>;       // one split: choose_splits cuts from 512 keys up
+    a.tiles = p.tq;
+    a.splits = p.dq;
+    a.numel = p.rows;
+    a.o[0] = p.dq > 1 ? static_cast<void*>(part) : dq;
+    const dim3 grid((unsigned)(p.heads * p.tq * p.dq));
+    if (few) {
         static dfsfm::SmemAttr attr;
-        attr.ensure(reinterpret_cast<const void*>(&attn_dkdv_kernel<T, DP>), smem);
-        hipLaunchKernelGGL((attn_dkdv_kernel<T, DP>), dim3((unsigned)(p.heads * p.tk * p.dkdv)), dim3(64 * NW), smem, st, a);
-        if (p.dkdv > 1) {
-            const dim3 grid((unsigned)((nk / 4 + 255) / 256));
-            hipLaunchKernelGGL((attn_sum_kernel<T>), grid, dim3(256), 0, st, part, nk, p.dkdv, dk);
-            hipLaunchKernelGGL((attn_sum_kernel<T>), grid, dim3(256), 0, st, part + p.dkdv * nk, nk, p.dkdv, dv);
-        }
+        attr.ensure(reinterpret_cast<const void*>(&attn_dq_kernel<T, DP, true>), smem);
+        hipLaunchKernelGGL((attn_dq_kernel<T, DP, true>), grid, dim3(256), smem, st, a);
+    } else {
+        static dfsfm::SmemAttr attr;
+        attr.ensure(reinterpret_cast<const void*>(&attn_dq_kernel<T, DP, false>), smem);
+        hipLaunchKernelGGL((attn_delta_kernel<M>), dim3((unsigned)((rows + 31) / 32)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((attn_dq_kernel<T, DP, false>), grid, dim3(256), smem, st, a);
+    }
+    if (p.dq > 1)
+        hipLaunchKernelGGL((attn_sum_kernel<M>), dim3((unsigned)((p.rows / 4 + 255) / 256)), dim3(256), 0, st, part, p.rows, p.dq, dq);
+    return check_launch("dfsfm_cross_attention_backward");
+}
+
+template <typename T, int DP>
+int dkdv_dp(Attn a, const Plan& p, Mem<T>* dk, Mem<T>* dv, float* part, hipStream_t st) {
+    typedef Mem<T> M;
+    a.tiles = p.tk;
+    a.splits = p.dkdv;
+    a.numel = p.keys;
+    a.o[0] = p.dkdv > 1 ? static_cast<void*>(part) : dk;
+    a.o[1] = p.dkdv > 1 ? static_cast<void*>(part + p.dkdv * p.keys) : dv;
+    constexpr int NW = KEY_WAVES<T, DP>;
+    constexpr int smem = (4 * Lds<T, DP>::TILE + (NW == 8 ? NW * 32 * DP : 0)) * sizeof(Elem<T>) + 4 * ROWS<T, DP> * 4;
+    static dfsfm::SmemAttr attr;
+    attr.ensure(reinterpret_cast<const void*>(&attn_dkdv_kernel<T, DP>), smem);
+    hipLaunchKernelGGL((attn_dkdv_kernel<T, DP>), dim3((unsigned)(p.heads * p.tk * p.dkdv)), dim3(64 * NW), smem, st, a);
+    if (p.dkdv > 1) {
+        const dim3 grid((unsigned)((p.keys / 4 + 255) / 256));
+        hipLaunchKernelGGL((attn_sum_kernel<M>), grid, dim3(256), 0, st, part, p.keys, p.dkdv, dk);
+        hipLaunchKernelGGL((attn_sum_kernel<M>), grid, dim3(256), 0, st, part + p.dkdv * p.keys, p.keys, p.dkdv, dv);
     }
     return check_launch("dfsfm_cross_attention_backward");
 }
 
-template <typename T>
-int forward_any(const Attn& a, const Plan& p, void* out, hipStream_t st) {
-    const int dp = pad_dim(a.D);
-    return dp == 32 ? forward_dp<T, 32>(a, p, (T*)out, st) : dp == 64 ? forward_dp<T, 64>(a, p, (T*)out, st) : forward_dp<T, 128>(a, p, (T*)out, st);
-}
+// CALL with T the type `dtype` (fp32 in planes if `wide`) and DP the padded head dim
+#define DFSFM_ATTN_DIM(CALL, T)                      \
+    switch (pad_dim(a.D)) {                          \
+        case 32: { constexpr int DP = 32; return CALL; }   \
+        case 64: { constexpr int DP = 64; return CALL; }   \
+        default: { constexpr int DP = 128; return CALL; }  \
+    }
+#define DFSFM_ATTN_CALL(dtype, wide, CALL)                              \
+    if (dtype == DFSFM_BF16) { typedef bf16 T; DFSFM_ATTN_DIM(CALL, T) } \
+    if (dtype == DFSFM_F16) { typedef f16 T; DFSFM_ATTN_DIM(CALL, T) }   \
+    if (wide) { typedef X3 T; DFSFM_ATTN_DIM(CALL, T) }                  \
+    { typedef float T; DFSFM_ATTN_DIM(CALL, T) }
 
-template <typename T>
-int backward_any(const Attn& a, const Plan& p, void* dq, void* dk, void* dv, float* part, hipStream_t st) {
-    const int dp = pad_dim(a.D);
-    return dp == 32   ? backward_dp<T, 32>(a, p, (T*)dq, (T*)dk, (T*)dv, part, st)
-           : dp == 64 ? backward_dp<T, 64>(a, p, (T*)dq, (T*)dk, (T*)dv, part, st)
-                      : backward_dp<T, 128>(a, p, (T*)dq, (T*)dk, (T*)dv, part, st);
+int forward_any(const Attn& a, const Plan& p, int dtype, void* out, hipStream_t st) {
+    DFSFM_ATTN_CALL(dtype, p.xq, (forward_dp<T, DP>(a, p, out, st)))
+}
+int dq_any(const Attn& a, const Plan& p, int dtype, void* dq, float* part, hipStream_t st) {
+    DFSFM_ATTN_CALL(dtype, p.xq, (dq_dp<T, DP>(a, p, (Mem<T>*)dq, part, st)))
+}
+int dkdv_any(const Attn& a, const Plan& p, int dtype, void* dk, void* dv, float* part, hipStream_t st) {
+    DFSFM_ATTN_CALL(dtype, p.xk, (dkdv_dp<T, DP>(a, p, (Mem<T>*)dk, (Mem<T>*)dv, part, st)))
 }
 
 }  // namespace
 
 extern "C" size_t dfsfm_cross_attention_workspace(int N, int L, int S, int H, int Hkv, int D, int dtype) {
     if (N <= 0 || L <= 0 || S < 0 || H <= 0 || !shape_ok(N, L, S, H, Hkv, D)) return 0;
-    const Plan p(N, L, S, H, Hkv, D, dtype);
-    return p.fwd > 1 ? (size_t)p.fwd * N * L * H * (D + 2) * sizeof(float) : 0;
+    return Plan(N, L, S, H, Hkv, D, dtype).forward(D);
 }
 
 extern "C" int dfsfm_cross_attention(const void* q, int64_t qn, int64_t ql, int64_t qh, const void* k, int64_t kn, int64_t ks, int64_t kh,
@@ -912,32 +1135,27 @@ extern "C" int dfsfm_cross_attention(const void* q, int64_t qn, int64_t ql, int6
     if (!shape_ok(N, L, S, H, Hkv, D)) return DFSFM_E_UNSUPPORTED;
     if (dtype < DFSFM_F32 || dtype > DFSFM_F16 || !rows_ok(q, qn, ql, qh, D, dtype) || ((uintptr_t)out & 15)) return DFSFM_E_UNSUPPORTED;
     if (S > 0 && (!rows_ok(k, kn, ks, kh, D, dtype) || !rows_ok(v, vn, vs, vh, D, dtype))) return DFSFM_E_UNSUPPORTED;
-    if (workspace_bytes < dfsfm_cross_attention_workspace(N, L, S, H, Hkv, D, dtype)) return DFSFM_E_WORKSPACE;
+    const Plan p(N, L, S, H, Hkv, D, dtype);
+    if (workspace_bytes < p.forward(D) || (p.forward(D) > 0 && (!workspace || ((uintptr_t)workspace & 15)))) return DFSFM_E_WORKSPACE;
+    hipStream_t st = static_cast<hipStream_t>(stream_);
     Attn a{};
     a.q = {q, qn, ql, qh};
-    a.k = {k, kn, ks, kh};
-    a.v = {v, vn, vs, vh};
+    a.k = a.kt = {k, kn, ks, kh};
+    a.v = a.vt = {v, vn, vs, vh};
     a.lens = kv_lens;
     a.mask = kv_mask;
     a.lse = lse;
     a.N = N, a.L = L, a.S = S, a.H = H, a.G = H / Hkv, a.D = D, a.scale = scale;
-    a.numel = (int64_t)N * L * H * D;
-    const Plan p(N, L, S, H, Hkv, D, dtype);
-    a.o[0] = workspace;
-    a.ml = static_cast<float*>(workspace) + p.fwd * a.numel;
-    hipStream_t st = static_cast<hipStream_t>(stream_);
-    if (dtype == DFSFM_F32) return forward_any<float>(a, p, out, st);
-    if (dtype == DFSFM_BF16) return forward_any<bf16>(a, p, out, st);
-    if (dtype == DFSFM_F16) return forward_any<f16>(a, p, out, st);
-    return DFSFM_E_UNSUPPORTED;
+    a.numel = p.rows;
+    if (p.xq) make_planes(a.k, a.v, N, S, Hkv, D, workspace, a.kt, a.vt, a.plane_k, st);
+    a.o[0] = static_cast<char*>(workspace) + p.planes_k();
+    a.ml = static_cast<float*>(a.o[0]) + p.fwd * p.rows;
+    return forward_any(a, p, dtype, out, st);
 }
 
 extern "C" size_t dfsfm_cross_attention_backward_workspace(int N, int L, int S, int H, int Hkv, int D, int dtype) {
     if (N <= 0 || L < 0 || S < 0 || H <= 0 || !shape_ok(N, L, S, H, Hkv, D)) return 0;
-    const Plan p(N, L, S, H, Hkv, D, dtype);
-    const size_t nq = (size_t)N * L * H, nk = (size_t)N * S * Hkv * D;
-    const size_t a = p.dq > 1 ? p.dq * nq * D : 0, b = p.dkdv > 1 ? 2 * p.dkdv * nk : 0;
-    return (nq + (a > b ? a : b)) * sizeof(float);
+    return Plan(N, L, S, H, Hkv, D, dtype).backward(D);
 }
 
 extern "C" int dfsfm_cross_attention_backward(const void* dout, int64_t gn, int64_t gl, int64_t gh, const void* q, int64_t qn, int64_t ql,
@@ -954,23 +1172,30 @@ extern "C" int dfsfm_cross_attention_backward(const void* dout, int64_t gn, int6
     if (L > 0 && (!rows_ok(q, qn, ql, qh, D, dtype) || !rows_ok(dout, gn, gl, gh, D, dtype) || !rows_ok(out, on, ol, oh, D, dtype)))
         return DFSFM_E_UNSUPPORTED;
     if (S > 0 && (!rows_ok(k, kn, ks, kh, D, dtype) || !rows_ok(v, vn, vs, vh, D, dtype))) return DFSFM_E_UNSUPPORTED;
-    if (workspace_bytes < dfsfm_cross_attention_backward_workspace(N, L, S, H, Hkv, D, dtype)) return DFSFM_E_WORKSPACE;
+    const Plan p(N, L, S, H, Hkv, D, dtype);
+    if (workspace_bytes < p.backward(D) || (p.backward(D) > 0 && (!workspace || ((uintptr_t)workspace & 15)))) return DFSFM_E_WORKSPACE;
+    hipStream_t st = static_cast<hipStream_t>(stream_);
     Attn a{};
-    a.q = {q, qn, ql, qh};
-    a.k = {k, kn, ks, kh};
-    a.v = {v, vn, vs, vh};
-    a.dout = {dout, gn, gl, gh};
+    a.q = a.qt = {q, qn, ql, qh};
+    a.k = a.kt = {k, kn, ks, kh};
+    a.v = a.vt = {v, vn, vs, vh};
+    a.dout = a.dt = {dout, gn, gl, gh};
     a.out = {out, on, ol, oh};
     a.lens = kv_lens;
     a.mask = kv_mask;
     a.lse = const_cast<float*>(lse);
     a.N = N, a.L = L, a.S = S, a.H = H, a.G = H / Hkv, a.D = D, a.scale = scale;
-    const Plan p(N, L, S, H, Hkv, D, dtype);
     a.delta = static_cast<float*>(workspace);
-    float* part = a.delta + (int64_t)N * L * H;
-    hipStream_t st = static_cast<hipStream_t>(stream_);
-    if (dtype == DFSFM_F32) return backward_any<float>(a, p, dq, dk, dv, part, st);
-    if (dtype == DFSFM_BF16) return backward_any<bf16>(a, p, dq, dk, dv, part, st);
-    if (dtype == DFSFM_F16) return backward_any<f16>(a, p, dq, dk, dv, part, st);
-    return DFSFM_E_UNSUPPORTED;
+    char* scratch = static_cast<char*>(workspace) + p.delta(D);            // dq's first, then the other's
+    if (L > 0) {
+        if (p.xq) make_planes(a.k, a.v, N, S, Hkv, D, scratch, a.kt, a.vt, a.plane_k, st);
+        const int rc = dq_any(a, p, dtype, dq, reinterpret_cast<float*>(scratch + p.planes_k()), st);
+        if (rc != DFSFM_OK) return rc;
+    }
+    if (S > 0) {
+        a.kt = a.k, a.vt = a.v;
+        if (p.xk) make_planes(a.q, a.dout, N, L, H, D, scratch, a.qt, a.dt, a.plane_q, st);
+        return dkdv_any(a, p, dtype, dk, dv, reinterpret_cast<float*>(scratch + p.planes_q()), st);
+    }
+    return DFSFM_OK;
 }
