@@ -23,7 +23,6 @@ using dfsfm::mfma32_row;
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float NEG = -INFINITY;
-
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
@@ -246,7 +245,7 @@ struct Attn {
     const uint8_t* mask;                   // [N, S]
     void* o[2];                            // results (out, or dq, or dk and dv): dense, in T or, with splits, 32-bit partials
     float* lse;                            // [N, H, L]
-    float* ml;                             // forward partials: maximum, sum [splits][N, H, L][2]
+    f32x4* ml;                             // forward partials: reference, sum, sum of rounded weights [splits][N, H, L]
     float* delta;                          // [N, H, L]
     int64_t numel;                         // elements of one partial result
     int N, L, S, H, G, D, splits, tiles;
@@ -258,31 +257,32 @@ struct Attn {
 // idle: 1.11 ms against 0.82 for the forward pass of 4 x 4800 x 6400 (ragged) x 16 heads x 128.
 struct Job {
     int n, hk, tile, split;
-    __device__ __forceinline__ Job(const Attn& a) {
+    __device__ __forceinline__ Job(const Attn& a, int tiles, int splits) {
         const int hkv = a.H / a.G, heads = a.N * hkv;
-        tile = blockIdx.x % a.tiles;
-        const int rest = blockIdx.x / a.tiles, head = rest % heads;
+        tile = blockIdx.x % tiles;
+        const int rest = blockIdx.x / tiles, head = rest % heads;
         split = rest / heads;
         n = head / hkv;
         hk = head % hkv;
     }
+    __device__ __forceinline__ explicit Job(const Attn& a) : Job(a, a.tiles, a.splits) {}
     // The same for tiles of `rows` keys, the tiles with keys of every sequence first: workgroups go to XCDs by their number, so tiles that
     // have nothing to do must not lie between the others (4 x 6400 ragged keys: XCDs with four rounds of work beside ones with three).
-    __device__ __forceinline__ Job(const Attn& a, int rows) : Job(a) {
+    __device__ __forceinline__ Job(const Attn& a, int tiles, int splits, int rows) : Job(a, tiles, splits) {
         if (!a.lens || a.N > 64) return;
-        const int hkv = a.H / a.G, per = hkv * a.splits;
+        const int hkv = a.H / a.G, per = hkv * splits;
         unsigned id = blockIdx.x;
         for (int pass = 0; pass < 2; ++pass)
             for (int i = 0; i < a.N; ++i) {
-                const int with = (min(max(a.lens[i], 0), a.S) + rows - 1) / rows, tiles = pass ? a.tiles - with : with;
-                if (id < (unsigned)(tiles * per)) {
+                const int with = (min(max(a.lens[i], 0), a.S) + rows - 1) / rows, count = pass ? tiles - with : with;
+                if (id < (unsigned)(count * per)) {
                     n = i;
-                    tile = (pass ? with : 0) + id % tiles;
-                    hk = id / tiles % hkv;
-                    split = id / tiles / hkv;
+                    tile = (pass ? with : 0) + id % count;
+                    hk = id / count % hkv;
+                    split = id / count / hkv;
                     return;
                 }
-                id -= tiles * per;
+                id -= count * per;
             }
     }
 };
@@ -290,7 +290,7 @@ struct Job {
 __device__ __forceinline__ int valid_len(const Attn& a, int n) { return a.lens ? min(max(a.lens[n], 0), a.S) : a.S; }
 
 // A tile of NROWS rows x DP channels on its way from memory into LDS, by LDS-DMA: no register holds it and no vector instruction moves it.
-// Every thread fetches 16 bytes an instruction; the chunk order of Lds is applied to the source address.  Rows behind the last and channels
+// Every one of THREADS threads (the workgroup, or a wave for itself) fetches 16 bytes an instruction; the chunk order of Lds is applied to the source address.  Rows behind the last and channels
 // behind D lie outside the buffer descriptor and arrive as zeros.
 template <typename T, int DP, int NROWS, int THREADS>
 struct Dma {
@@ -298,10 +298,11 @@ struct Dma {
     static constexpr int CH = L::CH, PER = NROWS * CH / THREADS, RPI = THREADS / CH;   // instructions a plane, rows an instruction
     static_assert(NROWS * CH % THREADS == 0, "every thread fetches the same number of chunks");
     int64_t plane;
-    unsigned off, step, row_bytes, stride;
+    unsigned tid, off, step, row_bytes, stride;
     __device__ __forceinline__ Dma(int64_t stride_, int D, int64_t plane_) : plane(plane_), stride((unsigned)(stride_ * sizeof(Elem<T>))) {
         row_bytes = D * (unsigned)sizeof(Elem<T>);
-        off = threadIdx.x / CH * stride;
+        tid = threadIdx.x % THREADS;
+        off = tid / CH * stride;
         step = RPI * stride;
     }
     // rows base .. base + rows - 1 (rows > 0); base, rows and tile are the same in every lane
@@ -311,14 +312,14 @@ struct Dma {
     }
     __device__ __forceinline__ void issue_plane(const Elem<T>* base, int rows, Elem<T>* tile) const {
         typedef int i32x4 __attribute__((ext_vector_type(4)));
-        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const uint64_t at = reinterpret_cast<uint64_t>(base);
         const i32x4 rsrc = {__builtin_amdgcn_readfirstlane((int)at), __builtin_amdgcn_readfirstlane((int)(at >> 32) & 0xffff),
                             __builtin_amdgcn_readfirstlane((int)((unsigned)(min(rows, NROWS) - 1) * stride + row_bytes)), 0x00020000};
         const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) void*)tile) + wave * 1024;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const unsigned c = (threadIdx.x % CH ^ L::order(threadIdx.x / CH) ^ L::order(RPI * i & 15)) * 16;
+            const unsigned c = (tid % CH ^ L::order(tid / CH) ^ L::order(RPI * i & 15)) * 16;
             // channels behind D: an offset no descriptor reaches (strides are below 2^23 elements)
             const unsigned o = c < row_bytes ? off + step * i + c : 0xff000000u;
             // As assembly (it writes no register) because the compiler lets every LDS read wait for its own form of this load.  The waits:
@@ -380,16 +381,30 @@ __device__ __forceinline__ f32x16 rows16(const float* v, int lane) {
     return r;
 }
 
-// out is a mean of values of v, but its weights are rounded and their sum is not: with v at fp16's largest value the quotient can pass it by
-// 2^-11 and would round to infinity.  A value that close behind the range becomes the largest one; infinities in v stay.
+// sum + the 8 weights of an operand, as they were rounded.  out is divided by this sum and not by that of the weights before rounding: it
+// stays a mean of values of v (v at fp16's largest value gives that value, not infinity; a row that one key dominates is exact), while lse
+// keeps the 32-bit sum.  One instruction for two weights.
 template <typename T>
-__device__ __forceinline__ float within_range(float x) {
-    if constexpr (__is_same(T, f16)) return fabsf(x) < 65600.f ? fminf(fmaxf(x, -65504.f), 65504.f) : x;
-    return x;
+__device__ __forceinline__ float add_rounded(const Frag<T>& f, float sum) {
+    if constexpr (__is_same(T, bf16)) {
+        typedef bf16 v2 __attribute__((ext_vector_type(2)));
+        const v2 one = {(bf16)1.f, (bf16)1.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum = __builtin_amdgcn_fdot2_f32_bf16(v2{f[2 * j], f[2 * j + 1]}, one, sum, false);
+    } else if constexpr (__is_same(T, f16)) {
+        typedef f16 v2 __attribute__((ext_vector_type(2)));
+        const v2 one = {(f16)1.f, (f16)1.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum = __builtin_amdgcn_fdot2(v2{f[2 * j], f[2 * j + 1]}, one, sum, false);
+    }
+    return sum;
 }
+// whether a type's weights are rounded before their product
+template <typename T>
+constexpr bool ROUNDS = !__is_same(T, float) && !__is_same(T, X3);
 
 // Stores a transposed accumulator (channels x columns) to the dense row of this lane's column.
-template <typename T, int DB, bool MEAN = false>
+template <typename T, int DB>
 __device__ __forceinline__ void store_col(T* row, const f32x16 (&acc)[DB], float f, int D, int lane) {
 #pragma unroll
     for (int b = 0; b < DB; ++b)
@@ -399,7 +414,7 @@ __device__ __forceinline__ void store_col(T* row, const f32x16 (&acc)[DB], float
             if (d < D) {                    // D is a multiple of 8
                 float t[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) t[e] = MEAN ? within_range<T>(acc[b][4 * g + e] * f) : acc[b][4 * g + e] * f;
+                for (int e = 0; e < 4; ++e) t[e] = acc[b][4 * g + e] * f;
                 dfsfm::store_f32<T, 4>(row + d, 4, t);
             }
         }
@@ -443,6 +458,73 @@ struct ColumnScale {
 };
 
 // ---------------------------------------------------------------- forward
+__device__ __forceinline__ float inverse(float sum) { return sum > 0.f || sum != sum ? 1.f / sum : 0.f; }
+// log sum exp of a row from its reference (in powers of two) and its sum; -inf without keys
+__device__ __forceinline__ float log_sum(float m, float sum) { return fmaf(m == NEG ? 0.f : m, LN2, logf(sum)); }
+
+// A wave's 32 columns of queries on their way through the keys.
+template <typename T, int DP, int KT = ROWS<T, DP>>
+struct Softmax {
+    static constexpr int DB = DP / 32, KS = DP / 16;
+    f32x16 acc[DB];
+    float m = NEG, sum = 0.f, rsum = 0.f;   // reference in powers of two of scale * log2(e) * q k; sums of this lane's half of the keys
+    const float c;
+    __device__ __forceinline__ explicit Softmax(float scale) : c(scale * LOG2E) {
+#pragma unroll
+        for (int b = 0; b < DB; ++b) acc[b] = splat16(0.f);
+    }
+    __device__ __forceinline__ void tile(const Lds<T, DP>& lds, const Elem<T>* kt, const Elem<T>* vt, const Frag<T> (&qf)[KS], unsigned long long bits, int lane) {
+        f32x16 st[KT / 32];
+#pragma unroll
+        for (int b = 0; b < KT / 32; ++b) {
+            st[b] = splat16(0.f);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) st[b] = Mma<T>::run(lds.read_rows(kt, 32 * b, 16 * s), qf[s], st[b]);
+        }
+        if (bits != ALL_KEYS<KT>) {
+#pragma unroll
+            for (int b = 0; b < KT / 32; ++b) drop_keys(st[b], (unsigned)(bits >> 32 * b >> 4 * (lane >> 5)));
+        }
+        float t = NEG;
+#pragma unroll
+        for (int b = 0; b < KT / 32; ++b)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) t = fmaxf(t, st[b][j]);
+        t = fmaxf(t, dfsfm::from_xor32(t, lane)) * c;
+        // the reference follows the maximum once it is 8 behind: weights up to 2^8 lose nothing, and most tiles rescale nothing
+        if (__ballot(t > m + 8.f)) {
+            const float mn = t > m + 8.f ? t : m, f = m == NEG ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            sum *= f;
+            rsum *= f;
+#pragma unroll
+            for (int b = 0; b < DB; ++b)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) acc[b][j] *= f;
+        }
+        const float mm = m == NEG ? 0.f : m;
+#pragma unroll
+        for (int b = 0; b < KT / 32; ++b) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                st[b][j] = __builtin_amdgcn_exp2f(fmaf(st[b][j], c, -mm));
+                sum += st[b][j];
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const Frag<T> p = pack8<T>(st[b], u);
+                rsum = add_rounded<T>(p, rsum);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) acc[d] = Mma<T>::run(lds.read_cols(vt, 32 * b + 16 * u, 32 * d), p, acc[d]);
+            }
+        }
+    }
+    __device__ __forceinline__ void finish() {
+        sum = dfsfm::add_xor32(sum);
+        rsum = ROUNDS<T> ? dfsfm::add_xor32(rsum) : sum;
+    }
+};
+
 // 4 waves x 32 rows a workgroup; tiles of 64 keys, two in LDS.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_forward_kernel(const Attn a) {
@@ -475,11 +557,8 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_forward_kernel(const
         dv.issue(vb + s0 * a.vt.l, end - s0, vs + buf * TILE);
         mask = key_mask(a, job.n, s0);
     };
-    f32x16 acc[DB];
-#pragma unroll
-    for (int b = 0; b < DB; ++b) acc[b] = splat16(0.f);
-    float m = NEG, sum = 0.f;               // maximum of scale * log2(e) * q k, sum of this lane's half of the keys
-    const float c = a.scale * LOG2E;
+    Softmax<T, DP> sm(a.scale);
+    const bool mine = job.tile * 128 + wave * 32 < R;
     if (beg < end) fetch(beg, 0);
     int buf = 0;
     for (int s0 = beg; s0 < end; s0 += KT, buf ^= 1) {
@@ -493,63 +572,121 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_forward_kernel(const
             __syncthreads();
         }
         if (s0 + KT < end) fetch(s0 + KT, buf ^ 1);
-        if (bits == 0) continue;
-        f32x16 st[KT / 32];
-#pragma unroll
-        for (int b = 0; b < KT / 32; ++b) {
-            st[b] = splat16(0.f);
-#pragma unroll
-            for (int s = 0; s < KS; ++s) st[b] = Mma<T>::run(lds.read_rows(kt, 32 * b, 16 * s), qf[s], st[b]);
-        }
-        if (bits != ALL_KEYS<KT>) {
-#pragma unroll
-            for (int b = 0; b < KT / 32; ++b) drop_keys(st[b], (unsigned)(bits >> 32 * b >> 4 * (lane >> 5)));
-        }
-        float t = NEG;
-#pragma unroll
-        for (int b = 0; b < KT / 32; ++b)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) t = fmaxf(t, st[b][j]);
-        t = fmaxf(t, dfsfm::from_xor32(t, lane)) * c;
-        // the reference follows the maximum once it is 8 behind: weights up to 2^8 lose nothing, and most tiles rescale nothing
-        if (__ballot(t > m + 8.f)) {
-            const float mn = t > m + 8.f ? t : m, f = m == NEG ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
-            sum *= f;
-#pragma unroll
-            for (int b = 0; b < DB; ++b)
-#pragma unroll
-                for (int j = 0; j < 16; ++j) acc[b][j] *= f;
-        }
-        const float mm = m == NEG ? 0.f : m;
-#pragma unroll
-        for (int b = 0; b < KT / 32; ++b) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                st[b][j] = __builtin_amdgcn_exp2f(fmaf(st[b][j], c, -mm));
-                sum += st[b][j];
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const Frag<T> p = pack8<T>(st[b], u);
-#pragma unroll
-                for (int d = 0; d < DB; ++d) acc[d] = Mma<T>::run(lds.read_cols(vt, 32 * b + 16 * u, 32 * d), p, acc[d]);
-            }
-        }
+        if (bits != 0 && mine) sm.tile(lds, kt, vt, qf, bits, lane);
     }
-    sum = dfsfm::add_xor32(sum);
+    sm.finish();
     if (r >= R) return;
     const int64_t row = ((int64_t)job.n * a.L + l) * a.H + h, at = ((int64_t)job.n * a.H + h) * a.L + l;
     if (a.splits > 1) {
-        store_col<float, DB>(static_cast<float*>(a.o[0]) + job.split * a.numel + row * a.D, acc, 1.f, a.D, lane);
-        if (lane < 32) {
-            float* ml = a.ml + ((int64_t)job.split * a.N * a.H * a.L + at) * 2;
-            ml[0] = m;
-            ml[1] = sum;
-        }
+        store_col<float, DB>(static_cast<float*>(a.o[0]) + job.split * a.numel + row * a.D, sm.acc, 1.f, a.D, lane);
+        if (lane < 32) a.ml[(int64_t)job.split * a.N * a.H * a.L + at] = f32x4{sm.m, sm.sum, sm.rsum, 0.f};
     } else {
-        store_col<Mem<T>, DB, true>(static_cast<Mem<T>*>(a.o[0]) + row * a.D, acc, sum > 0.f || sum != sum ? 1.f / sum : 0.f, a.D, lane);
-        if (lane < 32) a.lse[at] = fmaf(m == NEG ? 0.f : m, LN2, logf(sum));
+        store_col<Mem<T>, DB>(static_cast<Mem<T>*>(a.o[0]) + row * a.D, sm.acc, inverse(sm.rsum), a.D, lane);
+        if (lane < 32) a.lse[at] = log_sum(sm.m, sm.sum);
+    }
+}
+
+// Up to 32 rows a head, the single-token form: bound by the keys' bytes.  Every wave walks its own tiles of 32 keys through its own ring in
+// LDS, without a barrier, as many tiles ahead as 16 KB hold (two workgroups a CU; 32 KB and one: 72 us against 56 below); the waves' results
+// meet in LDS at the end.  32 single tokens x 8192 keys x 8 x 64 fp16: 95 us, 5.6 TB/s; 16 x 10816 ragged keys: 56 us with the join, 3.6 TB/s
+// (the kernel above, whose four waves share each tile: 117 and 60).
+template <typename T, int DP>
+struct Few {
+    static constexpr int KT = 32, TILE = KT * DP, STAGE = 2 * TILE * sizeof(T);       // K and V
+    static constexpr int WAVES = STAGE > 16384 ? 2 : 4, STAGES = STAGE > 8192 ? 2 : 16384 / STAGE, PITCH = DP + 4;
+    static constexpr int RING = WAVES * STAGES * STAGE, JOIN = WAVES * 32 * (PITCH + 4) * 4;
+    static constexpr int SMEM = RING > JOIN ? RING : JOIN;
+};
+template <typename T, int DP>
+__global__ __launch_bounds__((64 * Few<T, DP>::WAVES)) void attn_forward_few_kernel(const Attn a) {
+    typedef Few<T, DP> F;
+    constexpr int DB = DP / 32, KS = DP / 16, KT = F::KT, TILE = F::TILE, NW = F::WAVES, NS = F::STAGES;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    // splits are as long in every sequence, so that those that are there take as long
+    const int per = ((a.S + KT * NW - 1) / (KT * NW) + a.splits - 1) / a.splits * KT * NW;
+    const Job job(a, a.splits, 1, max(per, 1));
+    const int split = job.tile;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    T* ring = reinterpret_cast<T*>(smem) + wave * NS * 2 * TILE;
+    const Lds<T, DP> lds(lane);
+    const int R = a.L * a.G, r = lane & 31, l = r / a.G, h = job.hk * a.G + r % a.G;
+    const int len = valid_len(a, job.n);
+    const int end = (int)min((int64_t)len, (int64_t)(split + 1) * per), beg = min(end, (int)min((int64_t)end, (int64_t)split * per) + wave * KT);
+    Frag<T> qf[KS];
+    const T* qp = static_cast<const T*>(a.q.p) + job.n * a.q.n + (int64_t)min(l, a.L - 1) * a.q.l + h * a.q.h;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        const int c = 16 * s + 8 * (lane >> 5);
+        qf[s] = r < R && c < a.D ? load8<T>(qp + c) : zero_frag<T>();
+    }
+    const T* kb = static_cast<const T*>(a.k.p) + job.n * a.k.n + job.hk * a.k.h;
+    const T* vb = static_cast<const T*>(a.v.p) + job.n * a.v.n + job.hk * a.v.h;
+    const Dma<T, DP, KT, 64> dk(a.k.l, a.D, 0), dv(a.v.l, a.D, 0);
+    constexpr int LOADS = dk.PER + dv.PER;
+    auto fetch = [&](int s0, int stage) {
+        T* at = ring + stage * 2 * TILE;
+        dk.issue(kb + s0 * a.k.l, end - s0, at);
+        dv.issue(vb + s0 * a.v.l, end - s0, at + TILE);
+    };
+    Softmax<T, DP, KT> sm(a.scale);
+    dma_landed();                           // q is here: from now on the counter counts tiles
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i)
+        if (beg + i * KT * NW < end) fetch(beg + i * KT * NW, i);
+    int stage = 0;
+    for (int s0 = beg; s0 < end; s0 += KT * NW) {
+        // the stage after the last in flight was read in the turn before; its reads are done, their results went into products
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        const int ahead = s0 + (NS - 1) * KT * NW;
+        if (ahead < end) {
+            fetch(ahead, stage ? stage - 1 : NS - 1);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * LOADS) : "memory");
+        } else {
+            dma_landed();
+        }
+        T* at = ring + stage * 2 * TILE;
+        const unsigned long long bits = key_bits<KT>(key_mask(a, job.n, s0), s0, end);
+        if (a.mask && bits != ALL_KEYS<KT>) {                 // a weight of 0 does not undo a NaN in v
+            for (int e = lane; e < TILE / lds.E; e += 64)
+                if (!(bits >> (e / lds.CH) & 1)) *reinterpret_cast<f32x4*>(at + TILE + e * lds.E) = f32x4{0.f, 0.f, 0.f, 0.f};
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+        if (bits != 0) sm.tile(lds, at, at + TILE, qf, bits, lane);
+        stage = stage + 1 == NS ? 0 : stage + 1;
+    }
+    sm.finish();
+    __syncthreads();                        // the rings are done with
+    float* o = reinterpret_cast<float*>(smem);                            // [waves][32 rows][PITCH]
+    f32x4* ml = reinterpret_cast<f32x4*>(o + NW * 32 * F::PITCH);         // [waves][32]
+    store_col<float, DB>(o + (wave * 32 + r) * F::PITCH, sm.acc, 1.f, DP, lane);
+    if (lane < 32) ml[wave * 32 + r] = f32x4{sm.m, sm.sum, sm.rsum, 0.f};
+    __syncthreads();
+    for (int e = threadIdx.x; e < R * (a.D / 4); e += 64 * NW) {
+        const int row = e / (a.D / 4), d = e % (a.D / 4) * 4;
+        float m = NEG, sum = 0.f, rsum = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) m = fmaxf(m, ml[w * 32 + row][0]);
+        const float mm = m == NEG ? 0.f : m;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const f32x4 t = ml[w * 32 + row], x = *reinterpret_cast<const f32x4*>(o + (w * 32 + row) * F::PITCH + d);
+            const float f = __builtin_amdgcn_exp2f(t[0] - mm);
+            sum = fmaf(t[1], f, sum);
+            rsum = fmaf(t[2], f, rsum);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[c] = fmaf(x[c], f, v[c]);
+        }
+        const int hh = job.hk * a.G + row % a.G;
+        const int64_t to = ((int64_t)job.n * a.L + row / a.G) * a.H + hh, at = ((int64_t)job.n * a.H + hh) * a.L + row / a.G;
+        if (a.splits > 1) {
+            *reinterpret_cast<f32x4*>(static_cast<float*>(a.o[0]) + split * a.numel + to * a.D + d) = v;
+            if (d == 0) a.ml[(int64_t)split * a.N * a.H * a.L + at] = f32x4{m, sum, rsum, 0.f};
+        } else {
+            const float f = inverse(rsum), t[4] = {v[0] * f, v[1] * f, v[2] * f, v[3] * f};
+            dfsfm::store_f32<T, 4>(static_cast<T*>(a.o[0]) + to * a.D + d, 4, t);
+            if (d == 0) a.lse[at] = log_sum(m, sum);
+        }
     }
 }
 
@@ -562,25 +699,28 @@ __global__ __launch_bounds__(256) void attn_join_few_kernel(const Attn a) {
     if (row >= rows) return;
     const int h = (int)(row % a.H);
     const int64_t nl = row / a.H, at = (nl / a.L * a.H + h) * a.L + nl % a.L;
-    float m = NEG, sum = 0.f;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.ml[(s * rows + at) * 2]);
+    float m = NEG, sum = 0.f, rsum = 0.f;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.ml[s * rows + at][0]);
     const float mm = m == NEG ? 0.f : m;
-    for (int s = 0; s < a.splits; ++s) sum += a.ml[(s * rows + at) * 2 + 1] * __builtin_amdgcn_exp2f(a.ml[(s * rows + at) * 2] - mm);
-    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+        const f32x4 t = a.ml[s * rows + at];
+        const float f = __builtin_amdgcn_exp2f(t[0] - mm);
+        sum = fmaf(t[1], f, sum);
+        rsum = fmaf(t[2], f, rsum);
+    }
+    const float inv = inverse(rsum);
     for (int d = (threadIdx.x & 7) * 4; d < a.D; d += 32) {
         float o[4] = {0.f, 0.f, 0.f, 0.f};
         for (int s = 0; s < a.splits; ++s) {
-            const float f = __builtin_amdgcn_exp2f(a.ml[(s * rows + at) * 2] - mm) * inv;
+            const float f = __builtin_amdgcn_exp2f(a.ml[s * rows + at][0] - mm) * inv;
             float t[4];
             dfsfm::load_f32<float, 4>(static_cast<const float*>(a.o[0]) + s * a.numel + row * a.D + d, t);
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[e] = fmaf(t[e], f, o[e]);
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = within_range<T>(o[e]);
         dfsfm::store_f32<T, 4>(static_cast<T*>(a.o[1]) + row * a.D + d, 4, o);
     }
-    if ((threadIdx.x & 7) == 0) a.lse[at] = fmaf(mm, LN2, logf(sum));
+    if ((threadIdx.x & 7) == 0) a.lse[at] = log_sum(m, sum);
 }
 
 // Joins more of them, a wave a row: the lanes share the splits' maxima and sums, then 4 channels and every SG-th split each.
@@ -592,14 +732,13 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const Attn a) {
     const int64_t rows = (int64_t)a.N * a.L * a.H, row = (int64_t)blockIdx.x * 4 + wave, at0 = min(row, rows - 1);
     const int h = (int)(at0 % a.H);
     const int64_t nl = at0 / a.H, at = (nl / a.L * a.H + h) * a.L + nl % a.L;
-    typedef float f32x2 __attribute__((ext_vector_type(2)));
-    const f32x2* ml = reinterpret_cast<const f32x2*>(a.ml) + at;
-    f32x2 v[MAX_SPLITS / 64];
-    float m = NEG, sum = 0.f;
+    const f32x4* ml = a.ml + at;
+    f32x4 v[MAX_SPLITS / 64];
+    float m = NEG, sum = 0.f, rsum = 0.f;
 #pragma unroll
     for (int i = 0; i < MAX_SPLITS / 64; ++i) {
         const int s = lane + 64 * i;
-        v[i] = s < a.splits ? ml[s * rows] : f32x2{NEG, 0.f};
+        v[i] = s < a.splits ? ml[s * rows] : f32x4{NEG, 0.f, 0.f, 0.f};
         m = fmaxf(m, v[i][0]);
     }
 #pragma unroll
@@ -609,10 +748,14 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const Attn a) {
     for (int i = 0; i < MAX_SPLITS / 64; ++i) {
         v[i][0] = __builtin_amdgcn_exp2f(v[i][0] - mm);
         sum = fmaf(v[i][1], v[i][0], sum);
+        rsum = fmaf(v[i][2], v[i][0], rsum);
         weight[wave][lane + 64 * i] = v[i][0];
     }
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
+    for (int o = 1; o < 64; o <<= 1) {
+        sum += __shfl_xor(sum, o);
+        rsum += __shfl_xor(rsum, o);
+    }
     __syncthreads();
     if (row >= rows) return;
     const int lanes = a.D <= 32 ? 8 : a.D <= 64 ? 16 : 32, d = lane % lanes * 4;
@@ -625,14 +768,14 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const Attn a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[e] = fmaf(t[e], f, o[e]);
         }
-    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    const float inv = inverse(rsum);
     for (int x = lanes; x < 64; x <<= 1)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], x);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = within_range<T>(o[e] * inv);
+    for (int e = 0; e < 4; ++e) o[e] *= inv;
     if (d < a.D && lane < lanes) dfsfm::store_f32<T, 4>(static_cast<T*>(a.o[1]) + row * a.D + d, 4, o);
-    if (lane == 0) a.lse[at] = fmaf(mm, LN2, logf(sum));
+    if (lane == 0) a.lse[at] = log_sum(m, sum);
 }
 
 // ---------------------------------------------------------------- backward
@@ -781,7 +924,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
             __syncthreads();
             clear(buf, bits);
             if (s0 + KT < end) fetch(s0 + KT, buf ^ 1);
-            if (bits) accumulate(buf, bits);
+            if (bits && job.tile * 128 + wave * 32 < R) accumulate(buf, bits);
         }
     }
     if (r >= R) return;
@@ -815,7 +958,7 @@ __global__ __launch_bounds__((64 * KEY_WAVES<T, DP>), (KEY_WAVES<T, DP> / 4)) vo
     Elem<T>* os = qs + 2 * TILE;
     Elem<T>* vs = os + 2 * TILE;                                                // VLDS: the workgroup's keys
     float* rowv = reinterpret_cast<float*>(vs + (VLDS ? NW * 32 * DP : 0));      // [2][2][64]: -lse / scale, -delta
-    const Job job(a, NW * 32);
+    const Job job(a, a.tiles, a.splits, NW * 32);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hkv = a.H / a.G;
     const Lds<T, DP> lds(lane);
     const int s = job.tile * (NW * 32) + wave * 32 + (lane & 31);
@@ -982,7 +1125,7 @@ int choose_splits(int64_t groups, int64_t length, int slots) {
 // The launches of a call, from its sizes alone.
 struct Plan {
     int heads, tq, tk, fwd, dq, dkdv;       // row tiles, key tiles, splits
-    bool xq, xk;                            // fp32 in three planes: the kernels that walk the keys, the one that walks the rows
+    bool few, xq, xk;                            // fp32 in three planes: the kernels that walk the keys, the one that walks the rows
     int64_t rows, keys;                     // elements of q (or out), of k
     Plan(int N, int L, int S, int H, int Hkv, int D, int dtype) {
         heads = N * Hkv;
@@ -993,9 +1136,11 @@ struct Plan {
         const int wave_keys = 32 * (dtype != DFSFM_F32 && pad_dim(D) == 128 ? KEY_WAVES<bf16, 128> : KEY_WAVES<bf16, 32>);
         tq = (int)((R + 127) / 128);
         tk = (S + wave_keys - 1) / wave_keys;
-        // One row tile a head reads its keys once, from memory: 2048 workgroups keep more loads under way, and a long sequence among short ones
-        // ends sooner (16 single tokens x 10816 ragged keys x 8 x 64 fp16: 4 splits 59 us, 14 splits 42, the rate of a large copy).
-        fwd = dq = choose_splits((int64_t)heads * tq, S, tq == 1 ? 2048 : 512);
+        few = R <= 32;
+        // Few rows read their keys once, from memory: about a workgroup a CU does without the join (256 heads x 8192 x 64 fp16: 95 us against
+        // 110 in two splits), below that two a CU (128 heads x 10816 ragged keys: 56 us in four splits, 66 in two, 57 in eight).
+        fwd = few && heads >= 200 ? 1 : choose_splits((int64_t)heads * tq, S, tq == 1 && !few ? 2048 : 512);
+        dq = choose_splits((int64_t)heads * tq, S, tq == 1 ? 2048 : 512);
         dkdv = choose_splits((int64_t)heads * tk, R, wave_keys == 256 ? 256 : 512);
         rows = (int64_t)N * L * H * D;
         keys = (int64_t)N * S * Hkv * D;
@@ -1003,7 +1148,7 @@ struct Plan {
     // bytes of workspaces
     size_t planes_k() const { return xq ? (size_t)keys * 12 : 0; }
     size_t planes_q() const { return xk ? (size_t)rows * 12 : 0; }
-    size_t forward(int D) const { return planes_k() + (fwd > 1 ? (size_t)fwd * (rows + rows / D * 2) * 4 : 0); }
+    size_t forward(int D) const { return planes_k() + (fwd > 1 ? (size_t)fwd * (rows + rows / D * 4) * 4 : 0); }
     size_t delta(int D) const { return ((size_t)(rows / D) * 4 + 15) / 16 * 16; }
     size_t backward(int D) const {
         const size_t a = planes_k() + (dq > 1 ? (size_t)dq * rows * 4 : 0), b = planes_q() + (dkdv > 1 ? (size_t)2 * dkdv * keys * 4 : 0);
@@ -1037,7 +1182,18 @@ int forward_dp(Attn a, const Plan& p, void* out, hipStream_t st) {
     a.tiles = p.tq;
     a.splits = p.fwd;
     if (p.fwd == 1) a.o[0] = out;
-    hipLaunchKernelGGL((attn_forward_kernel<T, DP>), dim3((unsigned)(p.heads * p.tq * p.fwd)), dim3(256), smem, st, a);
+    const dim3 grid((unsigned)(p.heads * p.tq * p.fwd));
+    bool done = false;
+    if constexpr (!__is_same(T, X3)) {
+        if (p.few) {
+            typedef Few<T, DP> F;
+            static dfsfm::SmemAttr few;
+            few.ensure(reinterpret_cast<const void*>(&attn_forward_few_kernel<T, DP>), F::SMEM);
+            hipLaunchKernelGGL((attn_forward_few_kernel<T, DP>), grid, dim3(64 * F::WAVES), F::SMEM, st, a);
+            done = true;
+        }
+    }
+    if (!done) hipLaunchKernelGGL((attn_forward_kernel<T, DP>), grid, dim3(256), smem, st, a);
     if (p.fwd > 1) {
         a.o[1] = out;
         const int64_t rows = (int64_t)a.N * a.L * a.H;
@@ -1149,7 +1305,7 @@ extern "C" int dfsfm_cross_attention(const void* q, int64_t qn, int64_t ql, int6
     a.numel = p.rows;
     if (p.xq) make_planes(a.k, a.v, N, S, Hkv, D, workspace, a.kt, a.vt, a.plane_k, st);
     a.o[0] = static_cast<char*>(workspace) + p.planes_k();
-    a.ml = static_cast<float*>(a.o[0]) + p.fwd * p.rows;
+    a.ml = reinterpret_cast<f32x4*>(static_cast<float*>(a.o[0]) + p.fwd * p.rows);
     return forward_any(a, p, dtype, out, st);
 }
 
