@@ -403,21 +403,38 @@ __device__ __forceinline__ float add_rounded(const Frag<T>& f, float sum) {
 template <typename T>
 constexpr bool ROUNDS = !__is_same(T, float) && !__is_same(T, X3);
 
-// Stores a transposed accumulator (channels x columns) to the dense row of this lane's column.
+// Stores a transposed accumulator (channels x columns) to the dense row of this lane's column.  A lane holds 4 of every 8 channels; in 16
+// bits its partner's 4 are swapped in for every second eight, so that each stores 16 bytes: half the write requests of 8-byte stores.
 template <typename T, int DB>
 __device__ __forceinline__ void store_col(T* row, const f32x16 (&acc)[DB], float f, int D, int lane) {
 #pragma unroll
-    for (int b = 0; b < DB; ++b)
+    for (int b = 0; b < DB; ++b) {
+        if constexpr (sizeof(T) == 2) {
+            typedef T v4 __attribute__((ext_vector_type(4)));
+            typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+            typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int d = 32 * b + 8 * g + 4 * (lane >> 5);
-            if (d < D) {                    // D is a multiple of 8
-                float t[4];
+            for (int g = 0; g < 4; g += 2) {
+                v4 x, y;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) t[e] = acc[b][4 * g + e] * f;
-                dfsfm::store_f32<T, 4>(row + d, 4, t);
+                for (int e = 0; e < 4; ++e) {
+                    x[e] = (T)(acc[b][4 * g + e] * f);
+                    y[e] = (T)(acc[b][4 * g + 4 + e] * f);
+                }
+                const u32x2 u = __builtin_bit_cast(u32x2, x), v = __builtin_bit_cast(u32x2, y);
+                // lower half: its own and its partner's eight g; upper half: eight g + 1
+                const auto p = __builtin_amdgcn_permlane32_swap(u[0], v[0], false, false), q = __builtin_amdgcn_permlane32_swap(u[1], v[1], false, false);
+                const int d = 32 * b + 8 * g + 8 * (lane >> 5);
+                if (d < D) *reinterpret_cast<u32x4*>(row + d) = u32x4{p[0], q[0], p[1], q[1]};         // D is a multiple of 8
+            }
+        } else {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int d = 32 * b + 8 * g + 4 * (lane >> 5);
+                if (d < D) *reinterpret_cast<f32x4*>(row + d) = f32x4{acc[b][4 * g] * f, acc[b][4 * g + 1] * f, acc[b][4 * g + 2] * f, acc[b][4 * g + 3] * f};
             }
         }
+    }
 }
 
 // The operand of a fp16 product whose factors may be far below 1 (p times a gradient): a power of two per column, taken from the largest
@@ -473,21 +490,30 @@ struct Softmax {
 #pragma unroll
         for (int b = 0; b < DB; ++b) acc[b] = splat16(0.f);
     }
+    // A tile's second half without keys (a short sequence's last tile) is left out: 4800 x 77 x 64 29 -> 26 us.  At D = 128 the second copy of
+    // the code costs the loop its registers.
     __device__ __forceinline__ void tile(const Lds<T, DP>& lds, const Elem<T>* kt, const Elem<T>* vt, const Frag<T> (&qf)[KS], unsigned long long bits, int lane) {
-        f32x16 st[KT / 32];
+        if (KT == 64 && DP < 128 && bits >> 32 == 0)
+            blocks<1>(lds, kt, vt, qf, bits, lane);
+        else
+            blocks<KT / 32>(lds, kt, vt, qf, bits, lane);
+    }
+    template <int NB>
+    __device__ __forceinline__ void blocks(const Lds<T, DP>& lds, const Elem<T>* kt, const Elem<T>* vt, const Frag<T> (&qf)[KS], unsigned long long bits, int lane) {
+        f32x16 st[NB];
 #pragma unroll
-        for (int b = 0; b < KT / 32; ++b) {
+        for (int b = 0; b < NB; ++b) {
             st[b] = splat16(0.f);
 #pragma unroll
             for (int s = 0; s < KS; ++s) st[b] = Mma<T>::run(lds.read_rows(kt, 32 * b, 16 * s), qf[s], st[b]);
         }
         if (bits != ALL_KEYS<KT>) {
 #pragma unroll
-            for (int b = 0; b < KT / 32; ++b) drop_keys(st[b], (unsigned)(bits >> 32 * b >> 4 * (lane >> 5)));
+            for (int b = 0; b < NB; ++b) drop_keys(st[b], (unsigned)(bits >> 32 * b >> 4 * (lane >> 5)));
         }
         float t = NEG;
 #pragma unroll
-        for (int b = 0; b < KT / 32; ++b)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int j = 0; j < 16; ++j) t = fmaxf(t, st[b][j]);
         t = fmaxf(t, dfsfm::from_xor32(t, lane)) * c;
@@ -504,7 +530,7 @@ struct Softmax {
         }
         const float mm = m == NEG ? 0.f : m;
 #pragma unroll
-        for (int b = 0; b < KT / 32; ++b) {
+        for (int b = 0; b < NB; ++b) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
                 st[b][j] = __builtin_amdgcn_exp2f(fmaf(st[b][j], c, -mm));
@@ -874,6 +900,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
     auto accumulate = [&](int buf, unsigned long long bits) {
 #pragma unroll
         for (int b = 0; b < KT / 32; ++b) {
+            if (b && bits >> 32 == 0) break;
             f32x16 ds[1];
             products(buf, b, bits, ds[0]);
             cs.apply(ds, acc);
@@ -905,6 +932,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
         for (int t = 0; t * KT < end; ++t)
             if (bits[t]) {
                 for (int b = 0; b < KT / 32; ++b) {
+                    if (b && bits[t] >> 32 == 0) break;
                     f32x16 ds;
                     products(t, b, bits[t], ds);
 #pragma unroll
@@ -959,7 +987,8 @@ __global__ __launch_bounds__((64 * KEY_WAVES<T, DP>), (KEY_WAVES<T, DP> / 4)) vo
     Elem<T>* vs = os + 2 * TILE;                                                // VLDS: the workgroup's keys
     float* rowv = reinterpret_cast<float*>(vs + (VLDS ? NW * 32 * DP : 0));      // [2][2][64]: -lse / scale, -delta
     const Job job(a, a.tiles, a.splits, NW * 32);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hkv = a.H / a.G;
+    // which of the workgroup's keys a wave has turns with the workgroup: waves without any are not all on one SIMD
+    const int lane = threadIdx.x & 63, wave = ((threadIdx.x >> 6) + blockIdx.x) % NW, hkv = a.H / a.G;
     const Lds<T, DP> lds(lane);
     const int s = job.tile * (NW * 32) + wave * 32 + (lane & 31);
     const int len = valid_len(a, job.n);
@@ -1068,20 +1097,17 @@ __global__ __launch_bounds__((64 * KEY_WAVES<T, DP>), (KEY_WAVES<T, DP> / 4)) vo
     }
 }
 
-// out = sum of the splits' partials, in their order
+// x = sum of the splits' partials, in their order; blockIdx.y 1: y, from the partials behind
 template <typename T>
-__global__ __launch_bounds__(256) void attn_sum_kernel(const float* __restrict__ part, int64_t numel, int splits, T* __restrict__ out) {
+__global__ __launch_bounds__(256) void attn_sum_kernel(const float* __restrict__ part, int64_t numel, int splits, T* __restrict__ x, T* __restrict__ y) {
     const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;      // D is a multiple of 8, so numel is
     if (e >= numel) return;
-    float o[4] = {0.f, 0.f, 0.f, 0.f};
+    part += blockIdx.y * splits * numel + e;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
-        float t[4];
-        dfsfm::load_f32<float, 4>(part + s * numel + e, t);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] += t[i];
-    }
-    dfsfm::store_f32<T, 4>(out + e, 4, o);
+    for (int s = 0; s < splits; ++s) o += *reinterpret_cast<const f32x4*>(part + s * numel);
+    const float t[4] = {o[0], o[1], o[2], o[3]};
+    dfsfm::store_f32<T, 4>((blockIdx.y ? y : x) + e, 4, t);
 }
 
 // The three planes of x (blockIdx.y 0) or y (1), [N, len, heads, D] fp32, dense: 8 channels a thread.
@@ -1227,7 +1253,7 @@ int dq_dp(Attn a, const Plan& p, Mem<T>* dq, float* part, hipStream_t st) {
         hipLaunchKernelGGL((attn_dq_kernel<T, DP, false>), grid, dim3(256), smem, st, a);
     }
     if (p.dq > 1)
-        hipLaunchKernelGGL((attn_sum_kernel<M>), dim3((unsigned)((p.rows / 4 + 255) / 256)), dim3(256), 0, st, part, p.rows, p.dq, dq);
+        hipLaunchKernelGGL((attn_sum_kernel<M>), dim3((unsigned)((p.rows / 4 + 255) / 256)), dim3(256), 0, st, part, p.rows, p.dq, dq, dq);
     return check_launch("dfsfm_cross_attention_backward");
 }
 
@@ -1245,9 +1271,7 @@ int dkdv_dp(Attn a, const Plan& p, Mem<T>* dk, Mem<T>* dv, float* part, hipStrea
     attr.ensure(reinterpret_cast<const void*>(&attn_dkdv_kernel<T, DP>), smem);
     hipLaunchKernelGGL((attn_dkdv_kernel<T, DP>), dim3((unsigned)(p.heads * p.tk * p.dkdv)), dim3(64 * NW), smem, st, a);
     if (p.dkdv > 1) {
-        const dim3 grid((unsigned)((p.keys / 4 + 255) / 256));
-        hipLaunchKernelGGL((attn_sum_kernel<M>), grid, dim3(256), 0, st, part, p.keys, p.dkdv, dk);
-        hipLaunchKernelGGL((attn_sum_kernel<M>), grid, dim3(256), 0, st, part + p.dkdv * p.keys, p.keys, p.dkdv, dv);
+        hipLaunchKernelGGL((attn_sum_kernel<M>), dim3((unsigned)((p.keys / 4 + 255) / 256), 2), dim3(256), 0, st, part, p.keys, p.dkdv, dk, dv);
     }
     return check_launch("dfsfm_cross_attention_backward");
 }
