@@ -1749,7 +1749,8 @@ def layernorm_backward(dy, x, mean, rstd, gamma, need_weights=True):
     gamma = _norm_affine("layernorm_backward", x, C, gamma)
     if mean.dtype != torch.float32 or rstd.dtype != torch.float32 or mean.shape != shape[:-1] or rstd.shape != shape[:-1]:
         raise _lib.DfsfmError("layernorm_backward: mean and rstd are what layernorm_forward returned for x")
-    mean, rstd = mean.contiguous(), rstd.contiguous()
+    if not (mean.is_contiguous() and rstd.is_contiguous()):
+        mean, rstd = mean.contiguous(), rstd.contiguous()
     x, ldx = _norm_rows(x, C)
     dy, lddy = _norm_rows(dy, C)
     rows = x.numel() // C
