@@ -1125,6 +1125,9 @@ __global__ __launch_bounds__(256) void attn_planes_kernel(const Tensor x, const 
 // ---------------------------------------------------------------- host
 int pad_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
+// 1 / scale and scale * log2(e) are 32-bit numbers
+bool scale_ok(float s) { return s >= 1e-20f && s <= 1e20f; }
+
 // 16-byte loads; offsets within a tile of 64 rows are 32-bit byte offsets; a row does not overlap the next
 bool rows_ok(const void* p, int64_t n, int64_t l, int64_t h, int D, int dtype) {
     const int64_t e = dtype == DFSFM_F32 ? 4 : 8;
@@ -1311,7 +1314,7 @@ extern "C" int dfsfm_cross_attention(const void* q, int64_t qn, int64_t ql, int6
                                      void* out, float* lse, int N, int L, int S, int H, int Hkv, int D, float scale, int dtype,
                                      void* workspace, size_t workspace_bytes, void* stream_) {
     if (N == 0 || L == 0 || H == 0) return DFSFM_OK;
-    if (!q || !out || !lse || (S > 0 && (!k || !v)) || N < 0 || L < 0 || S < 0 || H < 0 || !(scale > 0.f)) return DFSFM_E_BADARG;
+    if (!q || !out || !lse || (S > 0 && (!k || !v)) || N < 0 || L < 0 || S < 0 || H < 0 || !scale_ok(scale)) return DFSFM_E_BADARG;
     if (!shape_ok(N, L, S, H, Hkv, D)) return DFSFM_E_UNSUPPORTED;
     if (dtype < DFSFM_F32 || dtype > DFSFM_F16 || !rows_ok(q, qn, ql, qh, D, dtype) || ((uintptr_t)out & 15)) return DFSFM_E_UNSUPPORTED;
     if (S > 0 && (!rows_ok(k, kn, ks, kh, D, dtype) || !rows_ok(v, vn, vs, vh, D, dtype))) return DFSFM_E_UNSUPPORTED;
@@ -1345,7 +1348,7 @@ extern "C" int dfsfm_cross_attention_backward(const void* dout, int64_t gn, int6
                                               int H, int Hkv, int D, float scale, int dtype, void* workspace, size_t workspace_bytes,
                                               void* stream_) {
     if (N == 0 || H == 0 || (L == 0 && S == 0)) return DFSFM_OK;
-    if (N < 0 || L < 0 || S < 0 || H < 0 || !(scale > 0.f)) return DFSFM_E_BADARG;
+    if (N < 0 || L < 0 || S < 0 || H < 0 || !scale_ok(scale)) return DFSFM_E_BADARG;
     if ((L > 0 && (!dout || !q || !out || !lse || !dq)) || (S > 0 && (!k || !v || !dk || !dv))) return DFSFM_E_BADARG;
     if (!shape_ok(N, L, S, H, Hkv, D)) return DFSFM_E_UNSUPPORTED;
     if (dtype < DFSFM_F32 || dtype > DFSFM_F16 || (((uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15)) return DFSFM_E_UNSUPPORTED;

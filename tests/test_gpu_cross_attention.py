@@ -295,6 +295,148 @@ def test_cross_attention_graphs(built_lib, L):
             assert all(torch.equal(o[n], ref[n]) for n in ref)
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("mask", ["none", "lens", "both"])
+@pytest.mark.parametrize("shape", [(1, 1, 9001, 1, 1, 64), (6, 3, 5000, 8, 2, 128), (1, 4, 4500, 8, 1, 32), (70, 1, 1100, 2, 2, 48), (40, 1, 530, 8, 8, 16)])
+def test_cross_attention_single_tokens(built_lib, shape, mask, t):
+    """Few rows: many splits and few, more workgroups than fit at once, whole splits without keys, more sequences than are sorted."""
+    q, k, v, do, lens, km, there = make(*shape, t, mask, seed=sum(shape))
+    check(both(q, k, v, do, lens, km), q, k, v, do, there, shape[-1] ** -0.5, (shape, mask, t))
+
+
+@pytest.mark.parametrize("shape", [(1, 100, 150, 2, 2, 32), (1, 100, 150, 2, 1, 64), (1, 80, 90, 1, 1, 128), (2, 3, 300, 2, 2, 64)])
+def test_cross_attention_fp32_keeps_its_range(built_lib, shape):
+    """fp32's products run in three bf16 planes or on the 32-bit instruction: with values, or with gradients, times 2^80 or 2^-60 every result
+    scales with them to the bit (a plane's last bit lies 2^-24 below its value, far above 2^-126)."""
+    q, k, v, do, lens, km, _ = (None if x is None else x.to(DEV) for x in make(*shape, torch.float32, "none", 31))
+    ref = both(q, k, v, do, lens, km)
+    for f in (2.0 ** 80, 2.0 ** -60):
+        a = both(q, k, v * f, do, lens, km)
+        assert torch.equal(a["out"], ref["out"] * f) and torch.equal(a["dv"], ref["dv"]) and torch.equal(a["dq"], ref["dq"] * f)
+        b = both(q, k, v, do * f, lens, km)
+        assert all(torch.equal(b[n], ref[n] * f) for n in ("dq", "dk", "dv"))
+
+
+def test_cross_attention_infinite_values(built_lib):
+    """An infinite value of v makes the channel that it stands in infinite or NaN (a weight's lower planes, or a weight that fp16 rounds to 0,
+    times infinity is NaN) and touches no other, in every kernel of the forward pass."""
+    for t in TYPES:
+        for L, S, D in ((1, 700, 64), (200, 300, 32), (200, 60, 128)):
+            q, k, v = (torch.randn(s, device=DEV).to(t) for s in ((1, L, 2, D), (1, S, 2, D), (1, S, 2, D)))
+            ref, _ = ops.cross_attention(q, k, v)
+            v[0, 17, 1, 5] = float("inf")
+            out, _ = ops.cross_attention(q, k, v)
+            assert not bool(out[0, :, 1, 5].isfinite().any())
+            out[0, :, 1, 5] = ref[0, :, 1, 5]
+            assert torch.equal(out, ref)
+
+
+def test_layer_of_the_operators_together(built_lib):
+    """A cross-attention layer as a user trains it: norms, projections, rotary positions of image grids on q and k, attention over padded
+    states with shared key heads, residual; all gradients by the operators' own backward passes, against automatic differentiation in 64
+    bits.  Seven stages, each off by at most ~64 u of its terms, their cancellations within a factor of 8: 7 * 64 * 8 * 2^-24 = 2.1e-4 of
+    each result's 2-norm."""
+    g = torch.Generator().manual_seed(41)
+    N, hw, hwk, H, Hkv, D = 2, (12, 16), (9, 20), 4, 2, 32
+    L, S, C = hw[0] * hw[1], hwk[0] * hwk[1], H * D
+    def param(*s, f=1.0, o=0.0):
+        return torch.randn(s, generator=g) * f + o
+    x, enc, dy = param(N, L, C), param(N, S, C), param(N, L, C)
+    p = {"g1": param(C, f=0.2, o=1.0), "b1": param(C, f=0.2), "g2": param(C, f=0.2, o=1.0), "b2": param(C, f=0.2), "wq": param(C, C, f=C ** -0.5),
+         "wk": param(C, Hkv * D, f=C ** -0.5), "wv": param(C, Hkv * D, f=C ** -0.5), "wo": param(C, C, f=C ** -0.5)}
+    mask = torch.zeros((N, *hwk), dtype=torch.bool)
+    mask[0, :7, :20] = True
+    mask[1, :9, :13] = True
+    mask = mask.reshape(N, S)
+    inv, _ = ops.rotary_frequencies(D, axes=2, device="cpu")
+    grid = [torch.stack(torch.meshgrid(torch.arange(h), torch.arange(w), indexing="ij"), -1).reshape(-1, 2) for h, w in (hw, hwk)]
+
+    def turn(t, pos):
+        out = []
+        for a in range(2):
+            ang = pos[:, a].double()[:, None] * inv
+            u, v = t[..., 2 * a * 8:(2 * a + 1) * 8], t[..., (2 * a + 1) * 8:(2 * a + 2) * 8]
+            c, s = ang.cos()[None, :, None], ang.sin()[None, :, None]
+            out += [u * c - v * s, v * c + u * s]
+        return torch.cat(out, -1)
+
+    def norm(t, gm, b):
+        m = t.mean(-1, keepdim=True)
+        return (t - m) / (((t - m) ** 2).mean(-1, keepdim=True) + 1e-5).sqrt() * gm + b
+
+    P = {n: t.double().requires_grad_() for n, t in {**p, "x": x, "enc": enc}.items()}
+    h, e = norm(P["x"], P["g1"], P["b1"]), norm(P["enc"], P["g2"], P["b2"])
+    q = turn((h @ P["wq"]).reshape(N, L, H, D), grid[0])
+    k = turn((e @ P["wk"]).reshape(N, S, Hkv, D), grid[1]).repeat_interleave(2, 2)
+    v = (e @ P["wv"]).reshape(N, S, Hkv, D).repeat_interleave(2, 2)
+    a = (q.transpose(1, 2) @ k.permute(0, 2, 3, 1) * D ** -0.5).masked_fill(~mask[:, None, None], -math.inf).softmax(-1) @ v.transpose(1, 2)
+    y = P["x"] + a.transpose(1, 2).reshape(N, L, C) @ P["wo"]
+    want = dict(zip(P, torch.autograd.grad(y, list(P.values()), dy.double())))
+    want["y"] = y.detach()
+
+    d = {n: t.to(DEV) for n, t in {**p, "x": x, "enc": enc, "dy": dy, "mask": mask, "inv": inv, "gq": grid[0], "gk": grid[1]}.items()}
+
+    def step():
+        """One forward and backward pass; elementwise torch and its products between the operators."""
+        h, mh, rh = ops.layernorm_forward(d["x"], d["g1"], d["b1"])
+        e, me, re = ops.layernorm_forward(d["enc"], d["g2"], d["b2"])
+        q = ops.rotary((h @ d["wq"]).view(N, L, H, D), d["gq"], d["inv"], axes=2, inplace=True)
+        k = ops.rotary((e @ d["wk"]).view(N, S, Hkv, D), d["gk"], d["inv"], axes=2)
+        v = (e @ d["wv"]).view(N, S, Hkv, D)
+        a, lse = ops.cross_attention(q, k, v, kv_mask=d["mask"])
+        y = d["x"] + a.view(N, L, C) @ d["wo"]
+        da = (d["dy"] @ d["wo"].t().contiguous()).view(N, L, H, D)
+        dq, dk, dv = ops.cross_attention_backward(da, q, k, v, a, lse, kv_mask=d["mask"])
+        dq = ops.rotary_backward(dq, d["gq"], d["inv"], axes=2, inplace=True).view(N, L, C)
+        dk = ops.rotary_backward(dk, d["gk"], d["inv"], axes=2).view(N, S, Hkv * D)
+        dv = dv.view(N, S, Hkv * D)
+        dh = dq @ d["wq"].t().contiguous()
+        de = dk @ d["wk"].t().contiguous() + dv @ d["wv"].t().contiguous()
+        dx, dg1, db1 = ops.layernorm_backward(dh, d["x"], mh, rh, d["g1"])
+        denc, dg2, db2 = ops.layernorm_backward(de, d["enc"], me, re, d["g2"])
+
+        def weight(t, dt):
+            return t.reshape(-1, t.shape[-1]).t().contiguous() @ dt.reshape(-1, dt.shape[-1])
+        return {"y": y, "x": dx + d["dy"], "enc": denc, "g1": dg1, "b1": db1, "g2": dg2, "b2": db2, "wq": weight(h, dq), "wk": weight(e, dk),
+                "wv": weight(e, dv), "wo": weight(a.view(N, L, C), d["dy"])}
+
+    got = step()
+    for n, t in want.items():
+        off = float((got[n].double().cpu() - t).norm() / t.norm())
+        assert off < 2.1e-4, (n, off)
+
+
+def test_training_operators_in_a_graph(built_lib):
+    """The operators' forward and backward passes captured together, replayed on new inputs between eager steps of the same tensors."""
+    N, L, S, H, D = 2, 130, 200, 4, 64
+    x = torch.randn((N, L, H * D), device=DEV)
+    gamma, beta = torch.rand(H * D, device=DEV) + 0.5, torch.randn(H * D, device=DEV)
+    k, v, dy = (torch.randn(s, device=DEV) for s in ((N, S, H, D), (N, S, H, D), (N, L, H, D)))
+    pos, lens = torch.arange(L, device=DEV), torch.tensor([150, 90], dtype=torch.int32, device=DEV)
+    inv, _ = ops.rotary_frequencies(D, device=DEV)
+
+    def step():
+        h, m, r = ops.layernorm_forward(x, gamma, beta)
+        q = ops.rotary(h.view(N, L, H, D), pos, inv)
+        out, lse = ops.cross_attention(q, k, v, kv_lens=lens)
+        dq, dk, dv = ops.cross_attention_backward(dy, q, k, v, out, lse, kv_lens=lens)
+        dh = ops.rotary_backward(dq, pos, inv).view(N, L, H * D)
+        return (out, dk, dv, *ops.layernorm_backward(dh, x, m, r, gamma))
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(4):
+        x.mul_(1.1).add_(0.01 * i)
+        pos.add_(1000 * i)
+        lens.copy_(torch.tensor([200 - 60 * i, 7 * i], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
 def test_cross_attention_refusals(built_lib):
     q, k = torch.randn((2, 3, 4, 32), device=DEV), torch.randn((2, 5, 2, 32), device=DEV)
     out, lse = ops.cross_attention(q, k, k)
@@ -304,7 +446,7 @@ def test_cross_attention_refusals(built_lib):
            lambda: ops.cross_attention(*(torch.randn((2, 3, 4, 136), device=DEV),) * 3), lambda: ops.cross_attention(q.double(), k.double(), k.double()),
            lambda: ops.cross_attention(q, k, k, kv_lens=lens[:1]), lambda: ops.cross_attention(q, k, k, kv_lens=lens.float()),
            lambda: ops.cross_attention(q, k, k, kv_lens=lens.cpu()), lambda: ops.cross_attention(q, k, k, kv_mask=mask[:, :4]),
-           lambda: ops.cross_attention(q, k, k, scale=0.0), lambda: ops.cross_attention(q, k, k, scale=float("nan")),
+           lambda: ops.cross_attention(q, k, k, scale=0.0), lambda: ops.cross_attention(q, k, k, scale=1e-25), lambda: ops.cross_attention(q, k, k, scale=float("nan")),
            lambda: ops.cross_attention(q[0], k[0], k[0]), lambda: ops.cross_attention(q.clone().requires_grad_(), k, k),
            lambda: ops.cross_attention_backward(q[:, :2], q, k, k, out, lse), lambda: ops.cross_attention_backward(q.half(), q, k, k, out, lse),
            lambda: ops.cross_attention_backward(q, q, k, k, out, lse.transpose(1, 2)), lambda: ops.cross_attention_backward(q, q, k, k, out, lse.half())]
