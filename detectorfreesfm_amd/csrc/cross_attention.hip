@@ -226,6 +226,35 @@ __device__ __forceinline__ Frag<T> pack8(const f32x16& s, int t) {
         return f;
     }
 }
+// FINE kernels: 8 values as the sum of two operands.  16-bit weights (or gradients) are off by as much as a 16-bit result is, and a result of
+// rounded ones by sqrt(2) of that, which many results share out evenly and few do not.  Where few rows read their keys once, from memory, a
+// second product takes 0 - 4 % more time, and only the result's own rounding is left (single tokens x 10816 keys fp16: 3.0e-4 -> 2.1e-4 off in the 2-norm).
+// 7/8 of the value and the rest: the error is that of 1/8 of it, and both have its sign, so that an infinite factor stays what it is.
+template <typename T>
+struct Fine {
+    Frag<T> p, rest;
+    __device__ __forceinline__ Fine(const f32x16& s, int t) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = (T)(0.875f * s[8 * t + j]);
+        asm("" : "+v"(p));                  // one p: the compiler may round a tie once for the product and otherwise, fused, for the rest
+#pragma unroll
+        for (int j = 0; j < 8; ++j) rest[j] = (T)(s[8 * t + j] - (float)p[j]);
+    }
+    // acc + x s
+    __device__ __forceinline__ f32x16 times(const Frag<T>& x, const f32x16& acc) const { return Mma<T>::run(x, rest, Mma<T>::run(x, p, acc)); }
+};
+template <typename T>
+struct Packed {
+    Frag<T> p;
+    __device__ __forceinline__ Packed(const f32x16& s, int t) : p(pack8<T>(s, t)) {}
+    __device__ __forceinline__ f32x16 times(const Frag<T>& x, const f32x16& acc) const { return Mma<T>::run(x, p, acc); }
+};
+template <typename T, bool FINE>
+struct OperandOf { typedef Packed<T> type; };
+template <typename T>
+struct OperandOf<T, true> { typedef Fine<T> type; };
+template <typename T, bool FINE>
+using Operand = typename OperandOf<T, FINE>::type;
 
 // Waves a SIMD that the forward and dq kernels are compiled for: two (256 registers a wave), so that one wave's exponentials run beside the
 // other's products.  fp32 at D = 128 holds twice the operands and would spill.
@@ -480,7 +509,7 @@ __device__ __forceinline__ float inverse(float sum) { return sum > 0.f || sum !=
 __device__ __forceinline__ float log_sum(float m, float sum) { return fmaf(m == NEG ? 0.f : m, LN2, logf(sum)); }
 
 // A wave's 32 columns of queries on their way through the keys.
-template <typename T, int DP, int KT = ROWS<T, DP>>
+template <typename T, int DP, int KT = ROWS<T, DP>, bool FINE = false>
 struct Softmax {
     static constexpr int DB = DP / 32, KS = DP / 16;
     f32x16 acc[DB];
@@ -538,16 +567,16 @@ struct Softmax {
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const Frag<T> p = pack8<T>(st[b], u);
-                rsum = add_rounded<T>(p, rsum);
+                const Operand<T, FINE> p(st[b], u);
+                if constexpr (!FINE) rsum = add_rounded<T>(p.p, rsum);
 #pragma unroll
-                for (int d = 0; d < DB; ++d) acc[d] = Mma<T>::run(lds.read_cols(vt, 32 * b + 16 * u, 32 * d), p, acc[d]);
+                for (int d = 0; d < DB; ++d) acc[d] = p.times(lds.read_cols(vt, 32 * b + 16 * u, 32 * d), acc[d]);
             }
         }
     }
     __device__ __forceinline__ void finish() {
         sum = dfsfm::add_xor32(sum);
-        rsum = ROUNDS<T> ? dfsfm::add_xor32(rsum) : sum;
+        rsum = ROUNDS<T> && !FINE ? dfsfm::add_xor32(rsum) : sum;
     }
 };
 
@@ -654,7 +683,7 @@ __global__ __launch_bounds__((64 * Few<T, DP>::WAVES)) void attn_forward_few_ker
         dk.issue(kb + s0 * a.k.l, end - s0, at);
         dv.issue(vb + s0 * a.v.l, end - s0, at + TILE);
     };
-    Softmax<T, DP, KT> sm(a.scale);
+    Softmax<T, DP, KT, ROUNDS<T>> sm(a.scale);
     dma_landed();                           // q is here: from now on the counter counts tiles
 #pragma unroll
     for (int i = 0; i < NS - 1; ++i)
@@ -829,11 +858,13 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(const Attn a) {
 
 // dq: the forward kernel's frame, K read both ways.
 //
-// SHORT (up to 128 keys: both tiles stay in LDS) also computes delta, as the sum of p dp over the keys it is equal to.  The sum over the
-// channels of dout times the ROUNDED out is off by half a step of out, an error that all keys of a row share: over many keys it drowns in
-// the roundings of ds, over few it does not (dq of 4800 x 77 fp16: 3.2e-4 off in the 2-norm against 2.1e-4 that the output's rounding alone
-// costs).  Two of three products are then made twice, over two tiles at most; a pass over dout and out is saved.
-template <typename T, int DP, bool SHORT>
+// delta: GIVEN, or summed here from p dp over the keys, which it is equal to.  The sum over the channels of dout times the ROUNDED out is off
+// by half a step of out, an error that all keys of a row share: over many keys it drowns in the roundings of ds, over few it does not (dq of
+// 4800 x 77 fp16: 3.2e-4 off in the 2-norm, 2.9e-4 so, 2.1e-4 by the output's rounding alone).  Two of three products are then made twice;
+// up to two tiles of keys stay in LDS (RESIDENT: a pass over dout and out is saved), up to EXACT_KEYS keys are read TWICE.
+enum Delta { GIVEN, RESIDENT, TWICE };
+constexpr int EXACT_KEYS = 512;
+template <typename T, int DP, Delta DELTA, bool FINE>
 __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn a) {
     constexpr int DB = DP / 32, KS = DP / 16, TILE = Lds<T, DP>::TILE, KT = ROWS<T, DP>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -860,7 +891,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
     const int64_t at = ((int64_t)job.n * a.H + h) * a.L + l;
     const float c = a.scale * LOG2E, lse = r < R ? a.lse[at] : NEG;
     const float lse2 = lse == NEG ? INFINITY : lse * LOG2E;              // a row without keys has p = 0
-    float delta = !SHORT && r < R ? a.delta[at] : 0.f;
+    float delta = DELTA == GIVEN && r < R ? a.delta[at] : 0.f;
     const Elem<T>* kb = static_cast<const Elem<T>*>(a.kt.p) + job.n * a.kt.n + job.hk * a.kt.h;
     const Elem<T>* vb = static_cast<const Elem<T>*>(a.vt.p) + job.n * a.vt.n + job.hk * a.vt.h;
     const Dma<T, DP, KT, 256> dk(a.kt.l, a.D, a.plane_k), dv(a.vt.l, a.D, a.plane_k);
@@ -906,43 +937,63 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
             cs.apply(ds, acc);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const Frag<T> p = pack8<T>(ds[0], u);
+                const Operand<T, FINE> p(ds[0], u);
 #pragma unroll
-                for (int d = 0; d < DB; ++d)
-                    acc[d] = Mma<T>::run(lds.read_cols(ks + buf * TILE, 32 * b + 16 * u, 32 * d), p, acc[d]);
+                for (int d = 0; d < DB; ++d) acc[d] = p.times(lds.read_cols(ks + buf * TILE, 32 * b + 16 * u, 32 * d), acc[d]);
             }
         }
     };
-    if constexpr (SHORT) {
-        unsigned long long bits[2] = {0, 0};
-        unsigned masks[2] = {0, 0};
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-            if (t * KT < end) {
-                fetch(t * KT, t);
-                masks[t] = mask;
-            }
-        dma_landed();
-#pragma unroll
-        for (int t = 0; t < 2; ++t) bits[t] = key_bits<KT>(masks[t], t * KT, end);
-        __syncthreads();
-        clear(0, bits[0]);
-        clear(1, bits[1]);
+    if constexpr (DELTA != GIVEN) {
         float sum = 0.f;
-        for (int t = 0; t * KT < end; ++t)
-            if (bits[t]) {
-                for (int b = 0; b < KT / 32; ++b) {
-                    if (b && bits[t] >> 32 == 0) break;
-                    f32x16 ds;
-                    products(t, b, bits[t], ds);
+        auto add = [&](int buf, unsigned long long bits) {
+            for (int b = 0; b < KT / 32; ++b) {
+                if (b && bits >> 32 == 0) break;
+                f32x16 ds;
+                products(buf, b, bits, ds);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) sum += ds[j];
-                }
+                for (int j = 0; j < 16; ++j) sum += ds[j];
             }
-        delta = dfsfm::add_xor32(sum);
-        if (r < R && lane < 32) a.delta[at] = delta;
-        for (int t = 0; t * KT < end; ++t)
-            if (bits[t]) accumulate(t, bits[t]);
+        };
+        auto added = [&]() {
+            delta = dfsfm::add_xor32(sum);
+            if (r < R && lane < 32) a.delta[at] = delta;
+        };
+        if constexpr (DELTA == RESIDENT) {
+            unsigned long long bits[2] = {0, 0};
+            unsigned masks[2] = {0, 0};
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                if (t * KT < end) {
+                    fetch(t * KT, t);
+                    masks[t] = mask;
+                }
+            dma_landed();
+#pragma unroll
+            for (int t = 0; t < 2; ++t) bits[t] = key_bits<KT>(masks[t], t * KT, end);
+            __syncthreads();
+            clear(0, bits[0]);
+            clear(1, bits[1]);
+            for (int t = 0; t * KT < end; ++t)
+                if (bits[t]) add(t, bits[t]);
+            added();
+            for (int t = 0; t * KT < end; ++t)
+                if (bits[t]) accumulate(t, bits[t]);
+        } else {
+            const int tiles = (end + KT - 1) / KT;
+            if (tiles) fetch(0, 0);
+            else added();
+            for (int i = 0; i < 2 * tiles; ++i) {
+                const int s0 = (i < tiles ? i : i - tiles) * KT, buf = i & 1;
+                dma_landed();
+                const unsigned long long bits = key_bits<KT>(mask, s0, end);
+                __syncthreads();
+                clear(buf, bits);
+                if (i + 1 < 2 * tiles) fetch((i + 1 < tiles ? i + 1 : i + 1 - tiles) * KT, buf ^ 1);
+                if (i == tiles) added();
+                if (bits && i < tiles) add(buf, bits);
+                if (bits && i >= tiles) accumulate(buf, bits);
+            }
+        }
     } else {
         if (beg < end) fetch(beg, 0);
         int buf = 0;
@@ -973,7 +1024,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
 template <typename T, int DP>
 constexpr int KEY_WAVES = DP == 128 && sizeof(Mem<T>) == 2 ? 8 : 4;
 
-template <typename T, int DP>
+template <typename T, int DP, bool FINE>
 __global__ __launch_bounds__((64 * KEY_WAVES<T, DP>), (KEY_WAVES<T, DP> / 4)) void attn_dkdv_kernel(const Attn a) {
     constexpr int NW = KEY_WAVES<T, DP>, THREADS = 64 * NW;
     constexpr bool VLDS = NW == 8;
@@ -1048,14 +1099,14 @@ __global__ __launch_bounds__((64 * KEY_WAVES<T, DP>), (KEY_WAVES<T, DP> / 4)) vo
         // -lse / scale and -delta start the sums; a row without keys, or behind the last, gets a score of -inf: p = 0
         if (threadIdx.x < 2 * KT) {
             const bool in = (int)(threadIdx.x % KT) < rows;
-            vt[threadIdx.x] = threadIdx.x < KT ? (in && rv != NEG ? -rv * inv_scale : NEG) : (in ? -rv : 0.f);
+            vt[threadIdx.x] = threadIdx.x < KT ? (in && rv != NEG ? -rv * (ROUNDS<T> ? inv_scale : LOG2E) : NEG) : (in ? -rv : 0.f);
         }
         __syncthreads();
         if (it + 1 < end) fetch(it + 1, buf ^ 1);
         if (!mine) continue;
 #pragma unroll UNROLL
         for (int b = 0; b < KT / 32; ++b) {
-            f32x16 st = rows16(vt + 32 * b, lane);
+            f32x16 st = ROUNDS<T> ? rows16(vt + 32 * b, lane) : splat16(0.f);
             f32x16 ds[1];
             ds[0] = rows16(vt + KT + 32 * b, lane);
 #pragma unroll
@@ -1063,20 +1114,22 @@ __global__ __launch_bounds__((64 * KEY_WAVES<T, DP>), (KEY_WAVES<T, DP> / 4)) vo
                 st = Mma<T>::run(lds.read_rows(qt, 32 * b, 16 * x), kf[x], st);
                 ds[0] = Mma<T>::run(lds.read_rows(ot, 32 * b, 16 * x), VLDS ? lds.read_rows(vs, 32 * wave, 16 * x) : vf[VLDS ? 0 : x], ds[0]);
             }
+            // 32 bits: the sums start at 0 and lse is taken off at the end, in one rounding
+            const f32x16 off = ROUNDS<T> ? splat16(SHIFT) : rows16(vt + 32 * b, lane);
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-                st[j] = __builtin_amdgcn_exp2f(fmaf(st[j], c, SHIFT));
+                st[j] = __builtin_amdgcn_exp2f(fmaf(st[j], c, off[j]));
                 ds[0][j] *= st[j];
             }
             cs.apply(ds, dk);
             if constexpr (VLDS) __builtin_amdgcn_sched_barrier(0);       // with the loop above not unrolled: no register spilled
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const Frag<T> p = pack8<T>(st, u), g = pack8<T>(ds[0], u);
+                const Operand<T, FINE> p(st, u), g(ds[0], u);
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
-                    dv[d] = Mma<T>::run(lds.read_cols(ot, 32 * b + 16 * u, 32 * d), p, dv[d]);
-                    dk[d] = Mma<T>::run(lds.read_cols(qt, 32 * b + 16 * u, 32 * d), g, dk[d]);
+                    dv[d] = p.times(lds.read_cols(ot, 32 * b + 16 * u, 32 * d), dv[d]);
+                    dk[d] = g.times(lds.read_cols(qt, 32 * b + 16 * u, 32 * d), dk[d]);
                 }
             }
         }
@@ -1145,7 +1198,7 @@ int choose_splits(int64_t groups, int64_t length, int slots) {
     for (int s = 1; s <= most || s == 1; ++s) {
         const int64_t n = groups * s, places = (n + slots - 1) / slots * slots;
         const double f = (double)n / (double)places;
-        if (f > fill + 0.02) fill = f, best = s;
+        if (f > fill * 1.02) fill = f, best = s;
         if (fill >= 0.85) break;
     }
     return best;
@@ -1169,7 +1222,7 @@ struct Plan {
         // Few rows read their keys once, from memory: about a workgroup a CU does without the join (256 heads x 8192 x 64 fp16: 95 us against
         // 110 in two splits), below that two a CU (128 heads x 10816 ragged keys: 56 us in four splits, 66 in two, 57 in eight).
         fwd = few && heads >= 200 ? 1 : choose_splits((int64_t)heads * tq, S, tq == 1 && !few ? 2048 : 512);
-        dq = choose_splits((int64_t)heads * tq, S, tq == 1 ? 2048 : 512);
+        dq = S <= EXACT_KEYS ? 1 : choose_splits((int64_t)heads * tq, S, tq == 1 ? 2048 : 512);
         dkdv = choose_splits((int64_t)heads * tk, R, wave_keys == 256 ? 256 : 512);
         rows = (int64_t)N * L * H * D;
         keys = (int64_t)N * S * Hkv * D;
@@ -1239,21 +1292,34 @@ int dq_dp(Attn a, const Plan& p, Mem<T>* dq, float* part, hipStream_t st) {
     typedef Mem<T> M;
     const int64_t rows = p.rows / a.D;
     constexpr int smem = 4 * Lds<T, DP>::TILE * sizeof(Elem<T>);
-    const bool few = a.S <= 2 * ROWS<T, DP>;       // one split: choose_splits cuts from 512 keys up
     a.tiles = p.tq;
     a.splits = p.dq;
     a.numel = p.rows;
     a.o[0] = p.dq > 1 ? static_cast<void*>(part) : dq;
     const dim3 grid((unsigned)(p.heads * p.tq * p.dq));
-    if (few) {
-        static dfsfm::SmemAttr attr;
-        attr.ensure(reinterpret_cast<const void*>(&attn_dq_kernel<T, DP, true>), smem);
-        hipLaunchKernelGGL((attn_dq_kernel<T, DP, true>), grid, dim3(256), smem, st, a);
+    auto launch = [&](auto kernel, dfsfm::SmemAttr& attr) {
+        attr.ensure(reinterpret_cast<const void*>(kernel), smem);
+        hipLaunchKernelGGL(kernel, grid, dim3(256), smem, st, a);
+    };
+    static dfsfm::SmemAttr attr[6];
+    const bool fine = ROUNDS<T> && p.tq == 1;
+    if (a.S <= 2 * ROWS<T, DP>) {
+        if (fine)
+            launch(&attn_dq_kernel<T, DP, RESIDENT, ROUNDS<T>>, attr[0]);
+        else
+            launch(&attn_dq_kernel<T, DP, RESIDENT, false>, attr[1]);
+    } else if (ROUNDS<T> && a.S <= EXACT_KEYS) {
+        constexpr Delta HOW = ROUNDS<T> ? TWICE : GIVEN;
+        if (fine)
+            launch(&attn_dq_kernel<T, DP, HOW, ROUNDS<T>>, attr[2]);
+        else
+            launch(&attn_dq_kernel<T, DP, HOW, false>, attr[3]);
     } else {
-        static dfsfm::SmemAttr attr;
-        attr.ensure(reinterpret_cast<const void*>(&attn_dq_kernel<T, DP, false>), smem);
         hipLaunchKernelGGL((attn_delta_kernel<M>), dim3((unsigned)((rows + 31) / 32)), dim3(256), 0, st, a);
-        hipLaunchKernelGGL((attn_dq_kernel<T, DP, false>), grid, dim3(256), smem, st, a);
+        if (fine)
+            launch(&attn_dq_kernel<T, DP, GIVEN, ROUNDS<T>>, attr[4]);
+        else
+            launch(&attn_dq_kernel<T, DP, GIVEN, false>, attr[5]);
     }
     if (p.dq > 1)
         hipLaunchKernelGGL((attn_sum_kernel<M>), dim3((unsigned)((p.rows / 4 + 255) / 256)), dim3(256), 0, st, part, p.rows, p.dq, dq, dq);
@@ -1270,9 +1336,16 @@ int dkdv_dp(Attn a, const Plan& p, Mem<T>* dk, Mem<T>* dv, float* part, hipStrea
     a.o[1] = p.dkdv > 1 ? static_cast<void*>(part + p.dkdv * p.keys) : dv;
     constexpr int NW = KEY_WAVES<T, DP>;
     constexpr int smem = (4 * Lds<T, DP>::TILE + (NW == 8 ? NW * 32 * DP : 0)) * sizeof(Elem<T>) + 4 * ROWS<T, DP> * 4;
-    static dfsfm::SmemAttr attr;
-    attr.ensure(reinterpret_cast<const void*>(&attn_dkdv_kernel<T, DP>), smem);
-    hipLaunchKernelGGL((attn_dkdv_kernel<T, DP>), dim3((unsigned)(p.heads * p.tk * p.dkdv)), dim3(64 * NW), smem, st, a);
+    const dim3 grid((unsigned)(p.heads * p.tk * p.dkdv));
+    if (ROUNDS<T> && (p.few || a.S <= 32)) {
+        static dfsfm::SmemAttr attr;
+        attr.ensure(reinterpret_cast<const void*>(&attn_dkdv_kernel<T, DP, ROUNDS<T>>), smem);
+        hipLaunchKernelGGL((attn_dkdv_kernel<T, DP, ROUNDS<T>>), grid, dim3(64 * NW), smem, st, a);
+    } else {
+        static dfsfm::SmemAttr attr;
+        attr.ensure(reinterpret_cast<const void*>(&attn_dkdv_kernel<T, DP, false>), smem);
+        hipLaunchKernelGGL((attn_dkdv_kernel<T, DP, false>), grid, dim3(64 * NW), smem, st, a);
+    }
     if (p.dkdv > 1) {
         hipLaunchKernelGGL((attn_sum_kernel<M>), dim3((unsigned)((p.keys / 4 + 255) / 256), 2), dim3(256), 0, st, part, p.keys, p.dkdv, dk, dv);
     }

@@ -54,10 +54,13 @@ def make(N, L, S, H, Hkv, D, t, mask, seed, q_scale=1.5, g_scale=1.0):
     return q, k, v, do, lens, km, there
 
 
-def reference(q, k, v, do, there, scale, out_type, got_out=None):
-    """{name: (64-bit value, bound before the last rounding)}"""
+def reference(q, k, v, do, there, scale, out_type, got_out=None, fine=False):
+    """{name: (64-bit value, bound before the last rounding)}; fine: weights and ds as two operands, 7/8 and the rounded rest (ut / 8 off, 2^-3 +
+    2^-8 with the first one's rounding in the rest), and delta as the sum of p dp over the keys."""
     t = q.dtype
     ut = 0.0 if t == torch.float32 else torch.finfo(t).eps / 2
+    if fine:
+        ut = ut * (1 / 8 + 1 / 256)
     fp16 = t == torch.float16
     G = q.shape[2] // k.shape[2]
     N, L, H, D = q.shape
@@ -87,6 +90,8 @@ def reference(q, k, v, do, there, scale, out_type, got_out=None):
     e_delta = (DO.abs() * (ob + torch.finfo(t).eps / 2 * (out.abs() + ob) + (D + 2) * U * out.abs())).sum(-1, keepdim=True)
     if fp16:
         e_delta = e_delta + 2.0 ** -25 * DO.abs().sum(-1, keepdim=True)
+    if fine:
+        e_delta = (p * (e_dp + (3 * ep + (S + 10) * U) * dp.abs())).sum(-1, keepdim=True)
     eds = p * (e_dp + e_delta + 2 * U * (dp.abs() + delta.abs())) + ds.abs() * 3 * ep
     wide = eds + (ut + 2 * U) * (ds.abs() + eds)
     R = L * G
@@ -117,8 +122,8 @@ def both(q, k, v, do, lens, km, scale=None):
     return {"out": out, "lse": lse, "dq": dq, "dk": dk, "dv": dv}
 
 
-def check(got, q, k, v, do, there, scale, what):
-    ref = reference(q, k, v, do, there, scale, q.dtype)
+def check(got, q, k, v, do, there, scale, what, **kw):
+    ref = reference(q, k, v, do, there, scale, q.dtype, **kw)
     for name, (value, bound) in ref.items():
         close(got[name], value, bound if name == "lse" else rounded(value, bound, q.dtype), (name, what))
         assert got[name].dtype == (torch.float32 if name == "lse" else q.dtype)
@@ -302,6 +307,23 @@ def test_cross_attention_single_tokens(built_lib, shape, mask, t):
     """Few rows: many splits and few, more workgroups than fit at once, whole splits without keys, more sequences than are sorted."""
     q, k, v, do, lens, km, there = make(*shape, t, mask, seed=sum(shape))
     check(both(q, k, v, do, lens, km), q, k, v, do, there, shape[-1] ** -0.5, (shape, mask, t))
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("mask", ["none", "lens", "both"])
+@pytest.mark.parametrize("shape", [(40, 1, 4, 8, 8, 64), (6, 4, 20, 8, 1, 32), (6, 16, 100, 2, 1, 128), (6, 32, 300, 1, 1, 48), (2, 1, 512, 16, 16, 80)])
+def test_cross_attention_few_rows_round_their_results_alone(built_lib, shape, mask, t):
+    """Up to 32 rows a head: weights and ds lose nothing that shows beside the rounding of the results."""
+    q, k, v, do, lens, km, there = make(*shape, t, mask, seed=sum(shape) + 1)
+    check(both(q, k, v, do, lens, km), q, k, v, do, there, shape[-1] ** -0.5, (shape, mask, t), fine=True)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("shape", [(3, 1, 1896, 1, 1, 40), (1, 1, 513, 2, 2, 64), (1, 130, 1500, 1, 1, 32), (1, 2000, 40, 1, 1, 64), (2, 700, 1, 1, 1, 128)])
+def test_cross_attention_few_heads(built_lib, shape, t):
+    """Few workgroups without splits: the keys (or the rows) are shared out."""
+    q, k, v, do, lens, km, there = make(*shape, t, "lens", seed=4)
+    check(both(q, k, v, do, lens, km), q, k, v, do, there, shape[-1] ** -0.5, (shape, t))
 
 
 @pytest.mark.parametrize("shape", [(1, 100, 150, 2, 2, 32), (1, 100, 150, 2, 1, 64), (1, 80, 90, 1, 1, 128), (2, 3, 300, 2, 2, 64)])

@@ -92,6 +92,9 @@ def test_cross_attention_workspaces(built_lib):
     assert L.dfsfm_cross_attention_workspace(64, 4096, 1024, 8, 8, 64, BF16) == 0
     assert L.dfsfm_cross_attention_workspace(64, 4096, 1024, 8, 8, 64, F32) == 2 * 3 * 2 * 64 * 1024 * 8 * 64       # three bf16 planes of k and v
     assert L.dfsfm_cross_attention_workspace(1, 1, 4096, 1, 1, 12, F16) == 0
+    # a few heads are split too: partials of dq (one row), and of dk and dv (one block of keys), behind delta's 16 bytes a row
+    assert L.dfsfm_cross_attention_backward_workspace(3, 1, 4096, 1, 1, 40, F32) >= 16 + 8 * 3 * 40 * 4
+    assert L.dfsfm_cross_attention_backward_workspace(3, 4096, 40, 1, 1, 40, BF16) >= 8 * 3 * 40 * 40 * 4 * 2
 
 
 def test_ops_refuse_cpu_tensors(built_lib):
