@@ -1187,12 +1187,14 @@ bool rows_ok(const void* p, int64_t n, int64_t l, int64_t h, int D, int dtype) {
     return !((uintptr_t)p & 15) && n % e == 0 && l % e == 0 && h % e == 0 && l >= D && l < (1ll << 23);
 }
 
-// Splits of the long axis (`length` rows of it, 256 a split at least).  `slots` workgroups run at a time (512: two a CU); as long as they
-// number less than eight such rounds the last one's idle places count, and the smallest number of splits that fills 85 % of the places is taken: 608
+// Splits of the long axis (`length` rows of it, `least` a split).  `slots` workgroups run at a time (512: two a CU); as long as they number
+// less than eight such rounds the last one's idle places count, and the smallest number of splits that fills 85 % of the places is taken: 608
 // workgroups of the forward pass 2 x 4800 x 10816 x 8 x 32 fp32 take 1.21 ms, three splits of each 0.98 with the join.
-int choose_splits(int64_t groups, int64_t length, int slots) {
+// A join is 5 us, what 256 keys of 16 bits take a wave; of fp32's products (32 keys of 128 channels: 3 us in planes, 5 on the 32-bit
+// instruction) 64 keys are worth one: 33 x 1387 x 4 x 80 forward and gradient 140 -> 81 us, one row of 4 x 3271 keys 120 -> 76.
+int choose_splits(int64_t groups, int64_t length, int slots, int least) {
     if (groups <= 0 || groups >= 8 * slots) return 1;
-    const int64_t most = length / 256 < MAX_SPLITS ? length / 256 : MAX_SPLITS;
+    const int64_t most = length / least < MAX_SPLITS ? length / least : MAX_SPLITS;
     int best = 1;
     double fill = 0;
     for (int s = 1; s <= most || s == 1; ++s) {
@@ -1216,14 +1218,15 @@ struct Plan {
         xq = dtype == DFSFM_F32 && R > 64;
         xk = dtype == DFSFM_F32 && S > 64;
         const int wave_keys = 32 * (dtype != DFSFM_F32 && pad_dim(D) == 128 ? KEY_WAVES<bf16, 128> : KEY_WAVES<bf16, 32>);
+        const int least = dtype == DFSFM_F32 ? 64 : 256;
         tq = (int)((R + 127) / 128);
         tk = (S + wave_keys - 1) / wave_keys;
         few = R <= 32;
         // Few rows read their keys once, from memory: about a workgroup a CU does without the join (256 heads x 8192 x 64 fp16: 95 us against
         // 110 in two splits), below that two a CU (128 heads x 10816 ragged keys: 56 us in four splits, 66 in two, 57 in eight).
-        fwd = few && heads >= 200 ? 1 : choose_splits((int64_t)heads * tq, S, tq == 1 && !few ? 2048 : 512);
-        dq = S <= EXACT_KEYS ? 1 : choose_splits((int64_t)heads * tq, S, tq == 1 ? 2048 : 512);
-        dkdv = choose_splits((int64_t)heads * tk, R, wave_keys == 256 ? 256 : 512);
+        fwd = few && heads >= 200 ? 1 : choose_splits((int64_t)heads * tq, S, tq == 1 && !few ? 2048 : 512, least);
+        dq = S <= (dtype == DFSFM_F32 ? 128 : EXACT_KEYS) ? 1 : choose_splits((int64_t)heads * tq, S, tq == 1 ? 2048 : 512, least);
+        dkdv = choose_splits((int64_t)heads * tk, R, wave_keys == 256 ? 256 : 512, least);
         rows = (int64_t)N * L * H * D;
         keys = (int64_t)N * S * Hkv * D;
     }
