@@ -3,15 +3,21 @@
 //   forward   s = scale q k^T over the keys that are there, p = softmax(s), out = p v, lse = log sum exp(s); no key: out = 0, lse = -inf
 //   backward  delta = <dout, out>, ds = p (dout v^T - delta), dq = scale ds k, dk = scale ds^T q, dv = p^T dout
 //
-// All products run on 32 x 32 MFMA tiles with 32-bit accumulators; fp32 tensors use the 32-bit matrix instruction (no split, no loss of
-// range), bf16 and fp16 the 16-bit one.  A lane holds ONE column of the score tile: a query in the forward and dq kernels, a key in the
-// dk / dv kernel, so the running maximum, the sum and the scale of a query are per-lane values, and the accumulator registers of a score
-// tile are, in their order, the operand of the next product (its other operand is read from LDS with the same order of the inner index):
-// the scores never leave the registers.  The query heads that share a key head are rows of one problem: row r is (query r / G, head r % G).
+// All products run on 32 x 32 MFMA tiles with 32-bit accumulators: bf16 and fp16 tensors on the 16-bit instruction, fp32 on it too, as three
+// bf16 planes (X3), where many rows share a key, and on the 32-bit one where few do.  A lane holds ONE column of the score tile: a query in
+// the forward and dq kernels, a key in the dk / dv kernel, so the running maximum, the sum and the scale of a query are per-lane values, and
+// the accumulator registers of a score tile are, in their order, the operand of the next product (its other operand is read from LDS with the
+// same order of the inner index): the scores never leave the registers.  The query heads that share a key head are rows of one problem: row
+// r is (query r / G, head r % G).
 //
-// Keys that are not there (behind kv_lens, or where kv_mask is 0) are zeroed on their way into LDS and get a bias of -inf, whatever the
-// memory held; a tile without any is skipped.  Few rows: the keys (or, for dk / dv, the rows) are cut into splits that write 32-bit partial
-// results, joined in a fixed order by a second kernel.  No atomics.
+// Tiles come by LDS-DMA, the next one while this one is worked on.  Keys behind kv_lens are out of the DMA descriptor's range and arrive as
+// zeros; rows of LDS whose kv_mask is 0 are cleared; scores of both are set to -inf; a tile without any key is skipped.  Few rows: the keys
+// (or, for dk / dv, the rows) are cut into splits that write 32-bit partial results, joined in a fixed order by a second kernel.  No atomics.
+//
+// What bounds the large cases is the exponentials beside the products: a wave's VALU instructions run at half rate while the other wave of its
+// SIMD streams MFMAs.  4 x 4800 x 6400 keys (ragged) x 16 / 4 heads x 128 bf16: forward 0.73, dq 0.89, dk / dv 1.20 ms, in products 0.85,
+// 1.03 and 1.03 PFLOP/s, where a plain 8192^3 product of the library runs at 1.17; 2 x 4800 x 10816 x 8 x 32 fp32 forward 0.57 ms = 140
+// TFLOP/s (library: 154).
 #include "elem.h"
 
 namespace {
@@ -228,7 +234,7 @@ __device__ __forceinline__ Frag<T> pack8(const f32x16& s, int t) {
 }
 // FINE kernels: 8 values as the sum of two operands.  16-bit weights (or gradients) are off by as much as a 16-bit result is, and a result of
 // rounded ones by sqrt(2) of that, which many results share out evenly and few do not.  Where few rows read their keys once, from memory, a
-// second product takes 0 - 4 % more time, and only the result's own rounding is left (single tokens x 10816 keys fp16: 3.0e-4 -> 2.1e-4 off in the 2-norm).
+// second product takes 0 - 5 % more time, and only the result's own rounding is left (single tokens x 10816 keys fp16: 3.0e-4 -> 2.1e-4 off in the 2-norm).
 // 7/8 of the value and the rest: the error is that of 1/8 of it, and both have its sign, so that an infinite factor stays what it is.
 template <typename T>
 struct Fine {
@@ -1214,7 +1220,7 @@ struct Plan {
     Plan(int N, int L, int S, int H, int Hkv, int D, int dtype) {
         heads = N * Hkv;
         const int64_t R = (int64_t)L * (H / Hkv);
-        // Splitting k and v (or q and dout) costs 20 bytes an element and pays from 64 rows (or keys) a head on; fewer are bound by memory.
+        // Planes of k and v (or of q and dout) cost 20 bytes an element and pay from 64 rows (or keys) a head on; fewer are bound by memory.
         xq = dtype == DFSFM_F32 && R > 64;
         xk = dtype == DFSFM_F32 && S > 64;
         const int wave_keys = 32 * (dtype != DFSFM_F32 && pad_dim(D) == 128 ? KEY_WAVES<bf16, 128> : KEY_WAVES<bf16, 32>);

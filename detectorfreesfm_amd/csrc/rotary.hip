@@ -8,6 +8,9 @@
 // Angles are 64-bit up to the fraction of a turn that is left (32 bits would be off by 0.06 rad at position 1e6); sine and cosine of that
 // fraction are 32-bit.  The kernel is bound by HBM: x in, y out.  A thread holds the sines of VP pairs of one token and walks the heads
 // with them, so the 64-bit part is paid once a token and not once a head; loads and stores are 16 bytes wide where P allows.
+//
+// 131072 tokens x 16 heads x 128 (64 turned) bf16: 239 us = 4.5 TB/s (a large copy: 4.7); 19200 x 8 x 32 fp32, two axes: 8.8 us = 4.5 TB/s;
+// 16 tokens x 8 x 64: 3.6 us, a launch's latency.
 #include "elem.h"
 
 namespace {

@@ -1907,8 +1907,9 @@ def cross_attention(q, k, v, kv_lens=None, kv_mask=None, scale=None):
     """softmax(scale * q k^T) v of q [N, L, H, D] over states k, v [N, S, Hkv, D] of another length, fp32 / bf16 / fp16, D a multiple of 8
     up to 128, strided views OK (unit channel stride); query head h reads key head h // (H / Hkv).  Sequence n looks at its keys s <
     kv_lens[n] (int tensor on the device, clamped to 0 .. S) with kv_mask[n, s] true; what padded places hold, NaN included, does not
-    matter, and a sequence without keys gives zeros; an infinity that is looked at gives infinity or NaN where it enters.  ``scale`` (1e-20 to 1e20) defaults to D ** -0.5.  L = 1 is the single-token form: the keys are
-    split over the chip and joined.  Returns (out [N, L, H, D] dense, lse [N, H, L] fp32: the scores' log-sum-exp, -inf without keys)."""
+    matter, and a sequence without keys gives zeros; an infinity that is looked at gives infinity or NaN where it enters.  ``scale``
+    (1e-20 to 1e20) defaults to D ** -0.5.  L = 1 is the single-token form: the keys are split over the chip and joined.  Returns (out
+    [N, L, H, D] dense, lse [N, H, L] fp32: the scores' log-sum-exp, -inf without keys)."""
     q, k, v, lens, mask, hold, scale, sizes, code = _attention_args("cross_attention", q, k, v, kv_lens, kv_mask, scale)
     N, L, S, H, Hkv, D = sizes
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
