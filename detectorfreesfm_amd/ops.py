@@ -5,6 +5,7 @@ hand-written gfx950 kernels from ``libdfsfm_hip.so``; none has a PyTorch/CPU fal
 """
 import ctypes
 import functools
+import inspect
 import os
 from typing import Optional
 
@@ -1657,14 +1658,17 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 def _on_first_device(fn):
     """``_on_device`` for operators whose first argument is a tensor: its device is made current if it is not; ``_operands`` refuses
     tensors elsewhere."""
+    first = next(iter(inspect.signature(fn).parameters))
+
     @functools.wraps(fn)
-    def wrapper(x, *args, **kw):
-        if not x.is_cuda:
-            raise _lib.DfsfmError("HIP ops need device tensors (there is no CPU path)")
+    def wrapper(*args, **kw):
+        x = args[0] if args else kw.get(first)
+        if not isinstance(x, torch.Tensor) or not x.is_cuda:
+            raise _lib.DfsfmError(f"{fn.__name__}: HIP ops need device tensors (there is no CPU path)")
         if x.get_device() == torch.cuda.current_device():
-            return fn(x, *args, **kw)
+            return fn(*args, **kw)
         with torch.cuda.device(x.get_device()):
-            return fn(x, *args, **kw)
+            return fn(*args, **kw)
     return wrapper
 
 

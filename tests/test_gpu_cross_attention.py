@@ -475,3 +475,11 @@ def test_cross_attention_refusals(built_lib):
     for call in bad:
         with pytest.raises(_lib.DfsfmError):
             call()
+
+
+def test_operands_by_name(built_lib):
+    q, k, w = torch.randn((2, 3, 4, 32), device=DEV), torch.randn((2, 5, 2, 32), device=DEV), torch.ones(32, device=DEV)
+    pos, (inv, _) = torch.arange(3, device=DEV), ops.rotary_frequencies(32, device=DEV)
+    assert all(torch.equal(a, b) for a, b in zip(ops.cross_attention(k=k, v=k, q=q, scale=0.2), ops.cross_attention(q, k, k, scale=0.2)))
+    assert all(torch.equal(a, b) for a, b in zip(ops.layernorm_forward(gamma=w, beta=w, x=q), ops.layernorm_forward(q, w, w)))
+    assert torch.equal(ops.rotary(positions=pos, inv_freq=inv, x=q), ops.rotary(q, pos, inv))

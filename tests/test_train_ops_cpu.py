@@ -107,6 +107,15 @@ def test_ops_refuse_cpu_tensors(built_lib):
             call()
 
 
+def test_first_operand_by_name(built_lib):
+    """The checks find the first operand where it is named, and say so where it is no tensor or is missing."""
+    x, w, h = torch.zeros(4, 64), torch.ones(64), torch.zeros(1, 4, 2, 32)
+    for call in (lambda: ops.layernorm_forward(x=x, gamma=w, beta=w), lambda: ops.cross_attention(k=h, v=h, q=h), lambda: ops.cross_attention(k=h, v=h),
+                 lambda: ops.rotary_backward(dy=h, positions=w, inv_freq=w), lambda: ops.cross_attention(None, h, h)):
+        with pytest.raises(_lib.DfsfmError, match="device tensors"):
+            call()
+
+
 def test_rotary_frequencies():
     inv, a = ops.rotary_frequencies(8, base=100.0, device="cpu")
     assert a == 1.0 and inv.dtype == torch.float64 and torch.allclose(inv, torch.tensor([1.0, 100 ** -0.25, 0.1, 100 ** -0.75], dtype=torch.float64), rtol=1e-15)
