@@ -483,3 +483,42 @@ def test_operands_by_name(built_lib):
     assert all(torch.equal(a, b) for a, b in zip(ops.cross_attention(k=k, v=k, q=q, scale=0.2), ops.cross_attention(q, k, k, scale=0.2)))
     assert all(torch.equal(a, b) for a, b in zip(ops.layernorm_forward(gamma=w, beta=w, x=q), ops.layernorm_forward(q, w, w)))
     assert torch.equal(ops.rotary(positions=pos, inv_freq=inv, x=q), ops.rotary(q, pos, inv))
+
+
+class Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, kv_lens, kv_mask):
+        out, lse = ops.cross_attention(q, k, v, kv_lens=kv_lens, kv_mask=kv_mask)
+        ctx.save_for_backward(q, k, v, out, lse, kv_lens, kv_mask)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, out, lse, kv_lens, kv_mask = ctx.saved_tensors
+        return *ops.cross_attention_backward(dout, q, k, v, out, lse, kv_lens=kv_lens, kv_mask=kv_mask), None, None
+
+
+@pytest.mark.parametrize("lowest", [True, False])
+@pytest.mark.parametrize("mask", ["none", "lens", "both"])
+def test_cross_attention_in_automatic_differentiation(built_lib, mask, lowest):
+    """Wrapped once as a function, the pair gives leaves the gradients of its direct calls: through an expanded gradient (of a sum), states
+    expanded over the batch, and leaves used twice.  lowest: the states keep the type's lowest value in places that the first sequence masks
+    and others see; a product with it passes fp32's range (3.4e38 times the sum of 32 values of q), and both sides are NaN there."""
+    q, k, v, _, lens, km, _ = (None if x is None else x.to(DEV) for x in make(3, 40, 70, 4, 2, 32, torch.float32, mask, 5))
+    k, v = torch.nan_to_num(k, 0.0, 0.0, 0.0), torch.nan_to_num(v, 0.0, 0.0, 0.0)
+    if not lowest:
+        k, v = (torch.where(x < -1e30, 0.0, x) for x in (k, v))
+    leaves = [x.clone().requires_grad_() for x in (q, k[:1], v[:1])]
+    kk, vv = (x.expand(3, 70, 2, 32) for x in leaves[1:])
+    (Attention.apply(leaves[0], kk, vv, lens, km).sum() + Attention.apply(leaves[0], kk, vv, lens, km).sum()).backward()
+    kk, vv = kk.detach(), vv.detach()
+    out, lse = ops.cross_attention(q, kk, vv, kv_lens=lens, kv_mask=km)
+    dq, dk, dv = ops.cross_attention_backward(torch.ones_like(out), q, kk, vv, out, lse, kv_lens=lens, kv_mask=km)
+    # twice a value is exact; three sequences' gradients are added in an order of torch's: two roundings of their absolute sum
+    def both_nan(a, b):
+        return torch.isnan(a) & torch.isnan(b) if lowest else torch.zeros_like(a, dtype=torch.bool)
+    assert bool(((leaves[0].grad == 2 * dq) | both_nan(leaves[0].grad, dq)).all())
+    for leaf, d in zip(leaves[1:], (dk, dv)):
+        d = d.double()
+        off = (leaf.grad.double() - 2 * d.sum(0, keepdim=True)).abs()
+        assert bool(((off <= 8 * U * d.abs().sum(0, keepdim=True)) | both_nan(leaf.grad, d.sum(0, keepdim=True))).all())
