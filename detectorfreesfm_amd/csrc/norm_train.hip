@@ -10,9 +10,9 @@
 // registers over all rows a lane group sees, then over the workgroup's groups in LDS, then over the workgroups by a second kernel: every
 // sum has a fixed order, no atomics.
 //
-// Time, kernels alone: 9600 x 256 fp32 forward with residual 6.4 us = 4.6 TB/s (a large copy: 4.7); 450000 x 128 fp32 forward 123 and
-// gradient 130 us = 4.7 and 4.4 TB/s (together with the weights' sums 256 us, the copy's time for those bytes is 245); 8192 x 4096 bf16
-// forward 26, gradient 42, weights' sums 5 us, 81 us a pass on inputs that are in no cache, where the five tensors of both take a copy 71.
+// Time, kernels alone: 9600 x 256 fp32 forward with residual 6.4 us = 4.6 TB/s (a copy of 2 GB: 4.7); 450000 x 128 fp32 forward 123 and
+// gradient 130 us = 5.6 and 5.3 TB/s (part of x comes from the last-level cache); 8192 x 4096 bf16 forward 26, gradient 42, weights' sums
+// 5 us, 81 us a pass on inputs that are in no cache, where the five tensors of both take a copy 71.
 #include "elem.h"
 
 namespace {
