@@ -234,7 +234,7 @@ __device__ __forceinline__ Frag<T> pack8(const f32x16& s, int t) {
 }
 // FINE kernels: 8 values as the sum of two operands.  16-bit weights (or gradients) are off by as much as a 16-bit result is, and a result of
 // rounded ones by sqrt(2) of that, which many results share out evenly and few do not.  Where few rows read their keys once, from memory, a
-// second product takes 0 - 5 % more time, and only the result's own rounding is left (single tokens x 10816 keys fp16: 3.0e-4 -> 2.1e-4 off in the 2-norm).
+// second product takes 0 - 8 % more time, and only the result's own rounding is left (single tokens x 10816 keys fp16: 3.0e-4 -> 2.1e-4 off in the 2-norm).
 // 7/8 of the value and the rest: the error is that of 1/8 of it, and both have its sign, so that an infinite factor stays what it is.
 template <typename T>
 struct Fine {
@@ -878,9 +878,14 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(const Attn a) {
 // delta: GIVEN, or summed here from p dp over the keys, which it is equal to.  The sum over the channels of dout times the ROUNDED out is off
 // by half a step of out, an error that all keys of a row share: over many keys it drowns in the roundings of ds, over few it does not (dq of
 // 4800 x 77 fp16: 3.2e-4 off in the 2-norm, 2.9e-4 so, 2.1e-4 by the output's rounding alone).  Two of three products are then made twice;
-// up to two tiles of keys stay in LDS (RESIDENT: a pass over dout and out is saved), up to EXACT_KEYS keys are read TWICE.
+// up to two tiles of keys stay in LDS (RESIDENT: a pass over dout and out is saved), up to EXACT_KEYS keys are read TWICE.  Where delta is
+// GIVEN and yet the keys may be few (a mask, up to FINE_KEYS of them, or one tile of rows), ds enters as two operands: dq of 248 rows x 7935
+// keys, a tenth of them there, bf16 2.6e-3 -> 1.8e-3 off (1.7e-3 by the output's rounding alone); 4 x 4800 x 4800 x 8 x 32 with a mask,
+// forward and gradient, 636 -> 687 us.
+template <bool B>
+struct Constant { static constexpr bool value = B; };
 enum Delta { GIVEN, RESIDENT, TWICE };
-constexpr int EXACT_KEYS = 512;
+constexpr int EXACT_KEYS = 512, FINE_KEYS = 2048;
 template <typename T, int DP, Delta DELTA, bool FINE>
 __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn a) {
     constexpr int DB = DP / 32, KS = DP / 16, TILE = Lds<T, DP>::TILE, KT = ROWS<T, DP>;
@@ -945,7 +950,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
 #pragma unroll
         for (int j = 0; j < 16; ++j) ds[j] *= __builtin_amdgcn_exp2f(fmaf(st[j], c, -lse2));
     };
-    auto accumulate = [&](int buf, unsigned long long bits) {
+    auto accumulate = [&](auto fine, int buf, unsigned long long bits) {
 #pragma unroll
         for (int b = 0; b < KT / 32; ++b) {
             if (b && bits >> 32 == 0) break;
@@ -954,12 +959,13 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
             cs.apply(ds, acc);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const Operand<T, FINE> p(ds[0], u);
+                const Operand<T, decltype(fine)::value> p(ds[0], u);
 #pragma unroll
                 for (int d = 0; d < DB; ++d) acc[d] = p.times(lds.read_cols(ks + buf * TILE, 32 * b + 16 * u, 32 * d), acc[d]);
             }
         }
     };
+    typedef Constant<FINE> Chosen;
     if constexpr (DELTA != GIVEN) {
         float sum = 0.f;
         auto add = [&](int buf, unsigned long long bits) {
@@ -994,7 +1000,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
                 if (bits[t]) add(t, bits[t]);
             added();
             for (int t = 0; t * KT < end; ++t)
-                if (bits[t]) accumulate(t, bits[t]);
+                if (bits[t]) accumulate(Chosen(), t, bits[t]);
         } else {
             const int tiles = (end + KT - 1) / KT;
             if (tiles) fetch(0, 0);
@@ -1008,20 +1014,26 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
                 if (i + 1 < 2 * tiles) fetch((i + 1 < tiles ? i + 1 : i + 1 - tiles) * KT, buf ^ 1);
                 if (i == tiles) added();
                 if (bits && i < tiles) add(buf, bits);
-                if (bits && i >= tiles) accumulate(buf, bits);
+                if (bits && i >= tiles) accumulate(Chosen(), buf, bits);
             }
         }
     } else {
-        if (beg < end) fetch(beg, 0);
-        int buf = 0;
-        for (int s0 = beg; s0 < end; s0 += KT, buf ^= 1) {
-            dma_landed();
-            const unsigned long long bits = key_bits<KT>(mask, s0, end);
-            __syncthreads();
-            clear(buf, bits);
-            if (s0 + KT < end) fetch(s0 + KT, buf ^ 1);
-            if (bits && job.tile * 128 + wave * 32 < R) accumulate(buf, bits);
-        }
+        auto walk = [&](auto fine) {
+            if (beg < end) fetch(beg, 0);
+            int buf = 0;
+            for (int s0 = beg; s0 < end; s0 += KT, buf ^= 1) {
+                dma_landed();
+                const unsigned long long bits = key_bits<KT>(mask, s0, end);
+                __syncthreads();
+                clear(buf, bits);
+                if (s0 + KT < end) fetch(s0 + KT, buf ^ 1);
+                if (bits && job.tile * 128 + wave * 32 < R) accumulate(fine, buf, bits);
+            }
+        };
+        if (ROUNDS<T> && !FINE && (a.mask || len <= FINE_KEYS))
+            walk(Constant<ROUNDS<T>>());
+        else
+            walk(Chosen());
     }
     if (r >= R) return;
     const int64_t row = ((int64_t)job.n * a.L + l) * a.H + h;

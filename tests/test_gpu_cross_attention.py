@@ -56,11 +56,12 @@ def make(N, L, S, H, Hkv, D, t, mask, seed, q_scale=1.5, g_scale=1.0):
 
 def reference(q, k, v, do, there, scale, out_type, got_out=None, fine=False):
     """{name: (64-bit value, bound before the last rounding)}; fine: weights and ds as two operands, 7/8 and the rounded rest (ut / 8 off, 2^-3 +
-    2^-8 with the first one's rounding in the rest), and delta as the sum of p dp over the keys."""
+    2^-8 with the first one's rounding in the rest), and delta as the sum of p dp over the keys; "ds": ds alone, of dq."""
     t = q.dtype
     ut = 0.0 if t == torch.float32 else torch.finfo(t).eps / 2
-    if fine:
-        ut = ut * (1 / 8 + 1 / 256)
+    uds = ut * (1 / 8 + 1 / 256) if fine else ut
+    if fine is True:
+        ut = uds
     fp16 = t == torch.float16
     G = q.shape[2] // k.shape[2]
     N, L, H, D = q.shape
@@ -90,12 +91,12 @@ def reference(q, k, v, do, there, scale, out_type, got_out=None, fine=False):
     e_delta = (DO.abs() * (ob + torch.finfo(t).eps / 2 * (out.abs() + ob) + (D + 2) * U * out.abs())).sum(-1, keepdim=True)
     if fp16:
         e_delta = e_delta + 2.0 ** -25 * DO.abs().sum(-1, keepdim=True)
-    if fine:
+    if fine is True:
         e_delta = (p * (e_dp + (3 * ep + (S + 10) * U) * dp.abs())).sum(-1, keepdim=True)
     eds = p * (e_dp + e_delta + 2 * U * (dp.abs() + delta.abs())) + ds.abs() * 3 * ep
     wide = eds + (ut + 2 * U) * (ds.abs() + eds)
     R = L * G
-    qb = wide @ K.abs() + (S + 8) * U * (ds.abs() @ K.abs())
+    qb = (eds + (uds + 2 * U) * (ds.abs() + eds)) @ K.abs() + (S + 8) * U * (ds.abs() @ K.abs())
     kb = wide.transpose(2, 3) @ Q.abs() + (R + 8) * U * (ds.abs().transpose(2, 3) @ Q.abs())
     vb = ((p * (3 * ep + ut + 2 * U)).transpose(2, 3) + (R + 8) * U * p.transpose(2, 3)) @ DO.abs()
     if fp16 and S:
@@ -316,6 +317,17 @@ def test_cross_attention_few_rows_round_their_results_alone(built_lib, shape, ma
     """Up to 32 rows a head: weights and ds lose nothing that shows beside the rounding of the results."""
     q, k, v, do, lens, km, there = make(*shape, t, mask, seed=sum(shape) + 1)
     check(both(q, k, v, do, lens, km), q, k, v, do, there, shape[-1] ** -0.5, (shape, mask, t), fine=True)
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape, mask", [((2, 300, 700, 2, 1, 32), "mask"), ((1, 129, 1500, 1, 1, 128), "both"), ((6, 200, 2048, 2, 2, 64), "lens"),
+                                         ((2, 100, 3000, 2, 2, 64), "none")])
+def test_cross_attention_dq_of_masked_keys(built_lib, shape, mask, t):
+    """dq of masked or few keys, or of one tile of rows, loses nothing by the rounding of ds."""
+    q, k, v, do, lens, km, there = make(*shape, t, mask, seed=sum(shape) + 2)
+    got = both(q, k, v, do, lens, km)
+    value, bound = reference(q, k, v, do, there, shape[-1] ** -0.5, t, fine="ds")["dq"]
+    close(got["dq"], value, rounded(value, bound, t), (shape, mask, t))
 
 
 @pytest.mark.parametrize("t", TYPES)
