@@ -1941,7 +1941,8 @@ def cross_attention_backward(dout, q, k, v, out, lse, kv_lens=None, kv_mask=None
         raise _lib.DfsfmError("cross_attention_backward: lse is what cross_attention returned, fp32 [N, H, L]")
     dout, out, lse = _heads(dout), _heads(out), lse.contiguous()
     dq = torch.empty_like(q, memory_format=torch.contiguous_format)
-    dk, dv = torch.empty_like(k, memory_format=torch.contiguous_format), torch.empty_like(v, memory_format=torch.contiguous_format)
+    states = torch.empty_like if H else torch.zeros_like         # the library writes nothing for no query heads: a sum over none is zero
+    dk, dv = states(k, memory_format=torch.contiguous_format), states(v, memory_format=torch.contiguous_format)
     lib = _lib.lib()
     nbytes = lib.dfsfm_cross_attention_backward_workspace(N, L, S, H, Hkv, D, code)
     ws = q.new_empty(nbytes, dtype=torch.uint8)

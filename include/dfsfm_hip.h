@@ -259,7 +259,7 @@ int dfsfm_cross_attention(const void* q, int64_t qn, int64_t ql, int64_t qh, con
 
 /* Its gradient for dout [N, L, H, D] from the forward pass's out and lse: dq [N, L, H, D], dk, dv [N, S, Hkv, D], dense, in the dtype; the
  * gradients of shared key heads are sums over their query heads; keys that are not there get zeros.  kv_lens, kv_mask and scale are the
- * forward pass's. */
+ * forward pass's.  H = 0 writes nothing: dk and dv, sums over no heads, are the caller's to clear. */
 size_t dfsfm_cross_attention_backward_workspace(int N, int L, int S, int H, int Hkv, int D, int dtype);
 int dfsfm_cross_attention_backward(const void* dout, int64_t gn, int64_t gl, int64_t gh, const void* q, int64_t qn, int64_t ql, int64_t qh,
                                    const void* k, int64_t kn, int64_t ks, int64_t kh, const void* v, int64_t vn, int64_t vs, int64_t vh,
