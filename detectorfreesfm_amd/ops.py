@@ -11,6 +11,7 @@ from typing import Optional
 
 import numpy as np
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import _lib
 
@@ -1678,6 +1679,8 @@ def _operands(what, x, same, others):
     if code is None:
         raise _lib.DfsfmError(f"{what}: need fp32, bf16 or fp16 tensors, got {x.dtype}")
     graph = torch.is_grad_enabled()
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (x, *same, *others)):
+        raise _lib.DfsfmError(f"{what}: an operand carries a tangent, which no operator here moves on: call it on the primal tensors")
     for t in (x, *same, *others):
         if t is None:
             continue
@@ -1871,9 +1874,9 @@ def _heads(t):
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _attention_args(what, q, k, v, kv_lens, kv_mask, scale, more=()):
+def _attention_args(what, q, k, v, kv_lens, kv_mask, scale, more=(), lse=None):
     """Checked tensors of a cross attention call: (q, k, v, pointers of kv_lens and kv_mask, what holds them, scale, sizes, type code)."""
-    code = _operands(what, q, (k, v, *more), (kv_lens, kv_mask))
+    code = _operands(what, q, (k, v, *more), (kv_lens, kv_mask, lse))
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
         raise _lib.DfsfmError(f"{what}: need q [N, L, H, D] and k, v [N, S, Hkv, D]")
     (N, L, H, D), (Nk, S, Hkv, Dk) = q.shape, k.shape
@@ -1933,11 +1936,11 @@ def cross_attention_backward(dout, q, k, v, out, lse, kv_lens=None, kv_mask=None
     """Gradients (dq, dk, dv), dense, of ``cross_attention`` for dout [N, L, H, D]; out and lse are what it returned, the other arguments
     what it was called with.  Keys that are not there get zeros.  Sums run in a fixed order: the same call gives the same bits.
     fp16: products p * ds are carried with a power of two per column, so gradients far below fp16's normal range keep their digits."""
-    q, k, v, lens, mask, hold, scale, sizes, code = _attention_args("cross_attention_backward", q, k, v, kv_lens, kv_mask, scale, (dout, out))
+    q, k, v, lens, mask, hold, scale, sizes, code = _attention_args("cross_attention_backward", q, k, v, kv_lens, kv_mask, scale, (dout, out), lse)
     N, L, S, H, Hkv, D = sizes
     if dout.shape != q.shape or out.shape != q.shape:
         raise _lib.DfsfmError("cross_attention_backward: dout and out have q's shape and type")
-    if lse.shape != (N, H, L) or lse.dtype != torch.float32 or lse.get_device() != q.get_device():
+    if lse.shape != (N, H, L) or lse.dtype != torch.float32:
         raise _lib.DfsfmError("cross_attention_backward: lse is what cross_attention returned, fp32 [N, H, L]")
     dout, out, lse = _heads(dout), _heads(out), lse.contiguous()
     dq = torch.empty_like(q, memory_format=torch.contiguous_format)

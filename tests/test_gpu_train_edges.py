@@ -3,8 +3,9 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
-from detectorfreesfm_amd import ops
+from detectorfreesfm_amd import _lib, ops
 from test_gpu_cross_attention import TYPES
 
 pytestmark = pytest.mark.gpu
@@ -22,3 +23,28 @@ def test_gradient_of_no_query_heads_is_zero(built_lib):
         dq, dk, dv = ops.cross_attention_backward(q, q, k, k, out, lse)
         assert dq.shape == q.shape and dk.shape == k.shape and dv.shape == k.shape
         assert bool((dk == 0).all()) and bool((dv == 0).all())
+
+
+def operator_calls():
+    """Every operator as a function of one tensor that it reads, and the tensor."""
+    x, w = torch.randn((4, 64), device=DEV), torch.ones(64, device=DEV)
+    h, k = torch.randn((2, 3, 4, 32), device=DEV), torch.randn((2, 5, 2, 32), device=DEV)
+    pos, (inv, _) = torch.arange(3, device=DEV), ops.rotary_frequencies(32, device=DEV)
+    _, m, r = ops.layernorm_forward(x, w, w)
+    out, lse = ops.cross_attention(h, k, k)
+    return [(x, lambda t: ops.layernorm_forward(t, w, w)), (w, lambda t: ops.layernorm_forward(x, t, w)), (w, lambda t: ops.layernorm_forward(x, w, t)),
+            (x, lambda t: ops.layernorm_forward(x, w, w, residual=t)), (x, lambda t: ops.layernorm_backward(t, x, m, r, w)),
+            (m, lambda t: ops.layernorm_backward(x, x, t, r, w)), (h, lambda t: ops.rotary(t, pos, inv)), (inv, lambda t: ops.rotary(h, pos, t)),
+            (h, lambda t: ops.rotary_backward(t, pos, inv)), (h, lambda t: ops.cross_attention(t, k, k)), (k, lambda t: ops.cross_attention(h, t, k)),
+            (k, lambda t: ops.cross_attention(h, k, t)), (h, lambda t: ops.cross_attention_backward(t, h, k, k, out, lse)),
+            (out, lambda t: ops.cross_attention_backward(h, h, k, k, t, lse)), (lse, lambda t: ops.cross_attention_backward(h, h, k, k, out, t))]
+
+
+def test_tangents_are_refused(built_lib):
+    """A dual tensor of forward-mode differentiation would lose its tangent without a word."""
+    for i, (x, call) in enumerate(operator_calls()):
+        with forward_ad.dual_level():
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(_lib.DfsfmError, match="tangent"):
+                    call(forward_ad.make_dual(x, torch.ones_like(x)))
+            call(x)                                                         # tensors without one pass
