@@ -1686,6 +1686,8 @@ def _operands(what, x, same, others):
             continue
         if t.get_device() != dev:
             raise _lib.DfsfmError(f"{what}: operands live on different devices, or not on a GPU")
+        if t.is_neg():
+            raise _lib.DfsfmError(f"{what}: an operand is a view whose sign is turned when it is read (of a conjugate): call resolve_neg() on it")
         if graph and t.requires_grad:
             raise _lib.DfsfmError(f"{what}: records no autograd graph: call it on detached tensors (or under torch.no_grad()) and its "
                                   "gradient with the backward function beside it")

@@ -48,3 +48,13 @@ def test_tangents_are_refused(built_lib):
                 with torch.set_grad_enabled(grad), pytest.raises(_lib.DfsfmError, match="tangent"):
                     call(forward_ad.make_dual(x, torch.ones_like(x)))
             call(x)                                                         # tensors without one pass
+
+
+def test_lazily_negated_tensors_are_refused(built_lib):
+    """The imaginary part of a conjugate is a view of the values before their sign is turned."""
+    for x, call in operator_calls():
+        turned = torch.complex(torch.zeros_like(x), -x).conj().imag
+        assert turned.is_neg() and torch.equal(turned, x)
+        with pytest.raises(_lib.DfsfmError, match="resolve_neg"):
+            call(turned)
+        call(turned.resolve_neg())

@@ -17,3 +17,14 @@ def test_operands_with_a_tangent():
                     ops._operands("call", *args)
         assert ops._operands("call", x, (x,), (None, x)) == 0
     assert ops._operands("call", x, (x,), (None, x)) == 0
+
+
+def test_lazily_negated_operands():
+    """The imaginary part of a conjugate lies in memory with the other sign."""
+    x = torch.ones(3)
+    turned = torch.complex(torch.zeros(3), -x).conj().imag
+    assert turned.is_neg() and torch.equal(turned, x)
+    for args in ((turned, (), ()), (x, (x, turned), (None,)), (x, (None,), (None, turned))):
+        with pytest.raises(_lib.DfsfmError, match="resolve_neg"):
+            ops._operands("call", *args)
+    assert ops._operands("call", turned.resolve_neg(), (x,), ()) == 0
