@@ -515,9 +515,15 @@ __device__ __forceinline__ float inverse(float sum) { return sum > 0.f || sum !=
 __device__ __forceinline__ float log_sum(float m, float sum) { return fmaf(m == NEG ? 0.f : m, LN2, logf(sum)); }
 
 // A wave's 32 columns of queries on their way through the keys.
+//
+// The reference m lies LIFT powers of two under the largest score it was taken from and follows once scores are 8 further above it.  fp16
+// weights then reach 2^15 and a row's largest is 2^7 or above: what rounds to a subnormal, by up to 2^-25, is off by 2^-32 of the largest.
+// With the reference at the largest score, weights under 2^-25 of it were 0: behind a first key that holds a row's weight, 9000 keys e^-17.5
+// below it came out up to a fifth off.
 template <typename T, int DP, int KT = ROWS<T, DP>, bool FINE = false>
 struct Softmax {
     static constexpr int DB = DP / 32, KS = DP / 16;
+    static constexpr float LIFT = __is_same(T, f16) ? 7.f : 0.f;
     f32x16 acc[DB];
     float m = NEG, sum = 0.f, rsum = 0.f;   // reference in powers of two of scale * log2(e) * q k; sums of this lane's half of the keys
     const float c;
@@ -553,8 +559,8 @@ struct Softmax {
             for (int j = 0; j < 16; ++j) t = fmaxf(t, st[b][j]);
         t = fmaxf(t, dfsfm::from_xor32(t, lane)) * c;
         // the reference follows the maximum once it is 8 behind: weights up to 2^8 lose nothing, and most tiles rescale nothing
-        if (__ballot(t > m + 8.f)) {
-            const float mn = t > m + 8.f ? t : m, f = m == NEG ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+        if (__ballot(t > m + (8.f + LIFT))) {
+            const float mn = t > m + (8.f + LIFT) ? t - LIFT : m, f = m == NEG ? 0.f : __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             sum *= f;
             rsum *= f;

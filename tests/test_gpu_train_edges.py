@@ -6,7 +6,7 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 from detectorfreesfm_amd import _lib, ops
-from test_gpu_cross_attention import TYPES
+from test_gpu_cross_attention import TYPES, U, close, rounded
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -58,3 +58,25 @@ def test_lazily_negated_tensors_are_refused(built_lib):
         with pytest.raises(_lib.DfsfmError, match="resolve_neg"):
             call(turned)
         call(turned.resolve_neg())
+
+
+@pytest.mark.parametrize("L, S, D, H", [(1, 60000, 32, 256), (1, 30000, 128, 256), (64, 30000, 64, 1800), (200, 9000, 32, 220), (200, 9000, 128, 220)])
+def test_fp16_weights_far_below_the_largest(built_lib, L, S, D, H):
+    """The first key holds nearly all of a row's weight and its value is 0: the result is what the many others add, each e^-16.5 to e^-18.5 of
+    it (fp16 numbers end at e^-16.6, and halves of that round to 0).  A weight is off by ut of itself and, below fp16's normal numbers, by
+    2^-25 of a scale on which the row's largest is 2^7 or above: 2^-32 of it.  out is divided by the sum of the same weights.  So many heads
+    that their keys are not split: a split without the first key has a largest weight of its own."""
+    g = torch.Generator().manual_seed(L + S)
+    q, k, v = torch.zeros((1, L, 1, D)), torch.zeros((1, S, 1, D)), torch.rand((1, S, 1, D), generator=g) + 0.5
+    q[..., 0] = 4.0
+    k[..., 0] = -17.5 / 4 + 0.5 * (torch.rand((1, S, 1), generator=g) - 0.5)
+    k[0, 0], v[0, 0] = 0.0, 0.0
+    q, k, v = q.half(), k.half(), v.half()
+    s = q[0, 0, 0].double() @ k[0, :, 0].double().T
+    p, V = torch.exp(s), v[0, :, 0].double()
+    out, total = p @ V / p.sum(), p.sum()
+    e = p * (2.0 ** -11 + 40 * U * (s.abs() + 1)) + 2.0 ** -32 + (S + 8) * U * p
+    bound = (e @ V + out * e.sum()) / total * (1 + 2.0 ** -8)
+    got, lse = ops.cross_attention(*(x.to(DEV).expand(-1, -1, H, -1) for x in (q, k, v)), scale=1.0)
+    close(got, out.expand(1, L, H, D), rounded(out, bound, torch.float16).expand(1, L, H, D), (L, S, D))
+    assert float((lse.double().cpu() - torch.log(total)).abs().max()) < (S + 40) * U
