@@ -27,7 +27,7 @@ struct RotaryArgs {
     const double* inv_freq;
     double turn;                // +-1 / 2 pi
     float amplitude;
-    unsigned tokens, L;
+    unsigned tokens, L, first;                // first: token of workgroup 0
     int H, D, pairs, axes, units, heads;      // units: threads a token; heads: heads a thread
 };
 
@@ -35,7 +35,7 @@ template <typename T, int VP, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
     constexpr int VC = 16 / sizeof(T);
     const unsigned per = 256u / a.units, sub = threadIdx.x / a.units;
-    const unsigned tok = blockIdx.x * per + sub;
+    const unsigned tok = a.first + blockIdx.x * per + sub;
     if (sub >= per || tok >= a.tokens) return;
     const int unit = threadIdx.x % a.units, turned = a.axes * a.pairs / VP;
     const int64_t n = tok / a.L, l = tok % a.L;
@@ -107,17 +107,23 @@ int rotary_launch(RotaryArgs a, bool interleaved, bool inplace, hipStream_t st) 
     // one thread a token and unit walks all heads where that leaves 2048 workgroups (eight a CU), fewer heads a thread otherwise
     const int slices = bx >= 2048 ? 1 : (int)((2048 + bx - 1) / bx);
     a.heads = (a.H + slices - 1) / slices;
-    const dim3 grid(bx, (unsigned)((a.H + a.heads - 1) / a.heads)), blk(256);
-#define DFSFM_ROT(VP_)                                                                            \
-    if (vp == VP_) {                                                                              \
-        if (interleaved)                                                                          \
-            hipLaunchKernelGGL((rotary_kernel<T, VP_, true>), grid, blk, 0, st, a);               \
-        else                                                                                      \
-            hipLaunchKernelGGL((rotary_kernel<T, VP_, false>), grid, blk, 0, st, a);              \
-    }
-    DFSFM_ROT(1) DFSFM_ROT(2) DFSFM_ROT(4)
-    if constexpr (VC == 8) DFSFM_ROT(8)
+    const dim3 blk(256);
+    // a launch holds less than 2^32 threads along an axis: from 2^24 workgroups on (16.8 M tokens of 256 units) the tokens take several
+    constexpr unsigned MOST = (1u << 24) - 1;
+    for (unsigned b = 0; b < bx; b += MOST) {
+        const dim3 grid(bx - b < MOST ? bx - b : MOST, (unsigned)((a.H + a.heads - 1) / a.heads));
+        a.first = b * per;
+#define DFSFM_ROT(VP_)                                                                                \
+        if (vp == VP_) {                                                                              \
+            if (interleaved)                                                                          \
+                hipLaunchKernelGGL((rotary_kernel<T, VP_, true>), grid, blk, 0, st, a);               \
+            else                                                                                      \
+                hipLaunchKernelGGL((rotary_kernel<T, VP_, false>), grid, blk, 0, st, a);              \
+        }
+        DFSFM_ROT(1) DFSFM_ROT(2) DFSFM_ROT(4)
+        if constexpr (VC == 8) DFSFM_ROT(8)
 #undef DFSFM_ROT
+    }
     return check_launch("dfsfm_rotary");
 }
 
@@ -134,7 +140,7 @@ extern "C" int dfsfm_rotary(const void* x, int64_t xn, int64_t xl, int64_t xh, v
     // 512 channels are at most 256 threads a token; the heads' slices are a grid axis of 16 bits
     if (D > 512 || axes > 2 || H > 65535 || L > 0x7fffffff || (int64_t)N * L > 0x7fffffff) return DFSFM_E_UNSUPPORTED;
     RotaryArgs a{x, xn, xl, xh, y, yn, yl, yh, positions, pn, pl, pa, inv_freq, (backward ? -1.0 : 1.0) * 0.15915494309189535,
-                 amplitude, (unsigned)(N * L), (unsigned)L, H, D, pairs, axes, 0, 0};
+                 amplitude, (unsigned)(N * L), (unsigned)L, 0, H, D, pairs, axes, 0, 0};
     hipStream_t st = static_cast<hipStream_t>(stream_);
     if (dtype == DFSFM_F32) return rotary_launch<float>(a, interleaved != 0, inplace, st);
     if (dtype == DFSFM_BF16) return rotary_launch<dfsfm::bf16>(a, interleaved != 0, inplace, st);

@@ -7,6 +7,7 @@ import torch.autograd.forward_ad as forward_ad
 
 from detectorfreesfm_amd import _lib, ops
 from test_gpu_cross_attention import TYPES, U, close, rounded
+from test_gpu_train_norm import rotary_reference
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -80,3 +81,18 @@ def test_fp16_weights_far_below_the_largest(built_lib, L, S, D, H):
     got, lse = ops.cross_attention(*(x.to(DEV).expand(-1, -1, H, -1) for x in (q, k, v)), scale=1.0)
     close(got, out.expand(1, L, H, D), rounded(out, bound, torch.float16).expand(1, L, H, D), (L, S, D))
     assert float((lse.double().cpu() - torch.log(total)).abs().max()) < (S + 40) * U
+
+
+def test_rotary_of_more_tokens_than_one_launch_holds(built_lib):
+    """2^24 and three tokens of 129 pairs of odd number, a workgroup each (8.7 GB): the same bits as in parts, and the turn of their positions
+    at the ends of the launches."""
+    L, P = (1 << 24) + 3, 129
+    x = torch.empty((1, L, 1, 2 * P), dtype=torch.float16, device=DEV).normal_()
+    pos, inv = torch.arange(L, device=DEV), torch.rand(P, dtype=torch.float64, device=DEV)
+    y = ops.rotary(x, pos, inv)
+    step = 1 << 21
+    assert all(torch.equal(y[:, i:i + step], ops.rotary(x[:, i:i + step], pos[i:i + step], inv)) for i in range(0, L, step))
+    for i in (0, (1 << 24) - 6, L - 4):
+        ref, bound = rotary_reference(x[:, i:i + 4].cpu(), pos[i:i + 4].cpu(), inv.cpu(), 1.0, 1, False, False)
+        close(y[:, i:i + 4], ref, rounded(ref, bound, torch.float16), i)
+    assert ops.rotary(x, pos, inv, inplace=True) is x and torch.equal(x, y)
