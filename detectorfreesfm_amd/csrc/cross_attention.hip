@@ -1276,12 +1276,14 @@ struct Plan {
     }
 };
 
-bool shape_ok(int N, int L, int S, int H, int Hkv, int D) {
+bool shape_ok(int N, int L, int S, int H, int Hkv, int D, bool backward) {
     if (D <= 0 || D > 128 || D % 8 || Hkv <= 0 || H % Hkv || (int64_t)H * D >= (1 << 23)) return false;
-    const int64_t R = (int64_t)L * (H / Hkv), heads = (int64_t)N * Hkv;
+    const int64_t R = (int64_t)L * (H / Hkv), heads = (int64_t)N * Hkv, tq = (R + 127) / 128, tk = ((int64_t)S + 127) / 128;
     // row and workgroup numbers are 32-bit
-    return R < (1ll << 30) && S < (1 << 30) && heads < (1 << 20) && heads * ((R + 127) / 128 + 2048) < (1ll << 31) &&
-           heads * (((int64_t)S + 127) / 128 + 2048) < (1ll << 31);
+    if (R >= (1ll << 30) || S >= (1 << 30) || heads >= (1 << 20) || heads * (tq + 2048) >= (1ll << 31) || heads * (tk + 2048) >= (1ll << 31)) return false;
+    // a launch holds less than 2^32 threads along an axis: of the attention kernels 256 a tile of 128 rows or keys, of delta's 8 a row (of the
+    // planes' one for 8 values: 2^32 of them have planes of 412 GB, more than there is)
+    return heads * tq < (1 << 24) && heads * tk < (1 << 24) && (!backward || heads * R < (1ll << 29));
 }
 
 // The planes of two tensors of the same sizes, dense, at `to`; the tensors as tiles are fetched from them.
@@ -1416,7 +1418,7 @@ int dkdv_any(const Attn& a, const Plan& p, int dtype, void* dk, void* dv, float*
 }  // namespace
 
 extern "C" size_t dfsfm_cross_attention_workspace(int N, int L, int S, int H, int Hkv, int D, int dtype) {
-    if (N <= 0 || L <= 0 || S < 0 || H <= 0 || !shape_ok(N, L, S, H, Hkv, D)) return 0;
+    if (N <= 0 || L <= 0 || S < 0 || H <= 0 || !shape_ok(N, L, S, H, Hkv, D, false)) return 0;
     return Plan(N, L, S, H, Hkv, D, dtype).forward(D);
 }
 
@@ -1426,7 +1428,7 @@ extern "C" int dfsfm_cross_attention(const void* q, int64_t qn, int64_t ql, int6
                                      void* workspace, size_t workspace_bytes, void* stream_) {
     if (N == 0 || L == 0 || H == 0) return DFSFM_OK;
     if (!q || !out || !lse || (S > 0 && (!k || !v)) || N < 0 || L < 0 || S < 0 || H < 0 || !scale_ok(scale)) return DFSFM_E_BADARG;
-    if (!shape_ok(N, L, S, H, Hkv, D)) return DFSFM_E_UNSUPPORTED;
+    if (!shape_ok(N, L, S, H, Hkv, D, false)) return DFSFM_E_UNSUPPORTED;
     if (dtype < DFSFM_F32 || dtype > DFSFM_F16 || !rows_ok(q, qn, ql, qh, D, dtype) || ((uintptr_t)out & 15)) return DFSFM_E_UNSUPPORTED;
     if (S > 0 && (!rows_ok(k, kn, ks, kh, D, dtype) || !rows_ok(v, vn, vs, vh, D, dtype))) return DFSFM_E_UNSUPPORTED;
     const Plan p(N, L, S, H, Hkv, D, dtype);
@@ -1448,7 +1450,7 @@ extern "C" int dfsfm_cross_attention(const void* q, int64_t qn, int64_t ql, int6
 }
 
 extern "C" size_t dfsfm_cross_attention_backward_workspace(int N, int L, int S, int H, int Hkv, int D, int dtype) {
-    if (N <= 0 || L < 0 || S < 0 || H <= 0 || !shape_ok(N, L, S, H, Hkv, D)) return 0;
+    if (N <= 0 || L < 0 || S < 0 || H <= 0 || !shape_ok(N, L, S, H, Hkv, D, true)) return 0;
     return Plan(N, L, S, H, Hkv, D, dtype).backward(D);
 }
 
@@ -1461,7 +1463,7 @@ extern "C" int dfsfm_cross_attention_backward(const void* dout, int64_t gn, int6
     if (N == 0 || H == 0 || (L == 0 && S == 0)) return DFSFM_OK;
     if (N < 0 || L < 0 || S < 0 || H < 0 || !scale_ok(scale)) return DFSFM_E_BADARG;
     if ((L > 0 && (!dout || !q || !out || !lse || !dq)) || (S > 0 && (!k || !v || !dk || !dv))) return DFSFM_E_BADARG;
-    if (!shape_ok(N, L, S, H, Hkv, D)) return DFSFM_E_UNSUPPORTED;
+    if (!shape_ok(N, L, S, H, Hkv, D, true)) return DFSFM_E_UNSUPPORTED;
     if (dtype < DFSFM_F32 || dtype > DFSFM_F16 || (((uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15)) return DFSFM_E_UNSUPPORTED;
     if (L > 0 && (!rows_ok(q, qn, ql, qh, D, dtype) || !rows_ok(dout, gn, gl, gh, D, dtype) || !rows_ok(out, on, ol, oh, D, dtype)))
         return DFSFM_E_UNSUPPORTED;

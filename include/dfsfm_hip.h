@@ -250,7 +250,9 @@ int dfsfm_rotary(const void* x, int64_t xn, int64_t xl, int64_t xh, void* y, int
  * null: all) with kv_mask[n, s] != 0 (uint8, dense [N, S]; null: all).  What k and v hold elsewhere is not looked at, NaN included; an
  * infinity that is looked at gives infinity or NaN where it enters.  A query without keys gets out = 0, lse = -inf.  Query head h reads
  * key head h / (H / Hkv); H is a multiple of Hkv, D a multiple of 8 up to 128, scale 1e-20 to 1e20.  Element strides n, length, head with
- * unit channel stride; rows lie on 16-byte boundaries, length strides are D to below 2^23; results and workspace on 16-byte boundaries. */
+ * unit channel stride; rows lie on 16-byte boundaries, length strides are D to below 2^23; results and workspace on 16-byte boundaries.
+ * Sizes: H * D below 2^23, N * Hkv below 2^20, tiles of 128 of a head's L * H / Hkv rows, or of its S keys, below 2^24 over all heads;
+ * more is DFSFM_E_UNSUPPORTED.  The gradient: N * L * H below 2^29 too. */
 size_t dfsfm_cross_attention_workspace(int N, int L, int S, int H, int Hkv, int D, int dtype);
 int dfsfm_cross_attention(const void* q, int64_t qn, int64_t ql, int64_t qh, const void* k, int64_t kn, int64_t ks, int64_t kh,
                           const void* v, int64_t vn, int64_t vs, int64_t vh, const int* kv_lens, const uint8_t* kv_mask, void* out,

@@ -4,6 +4,7 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 from detectorfreesfm_amd import _lib, ops
+from test_train_ops_cpu import UNSUPPORTED, WORKSPACE, attention, attention_backward
 
 
 def test_operands_with_a_tangent():
@@ -28,3 +29,20 @@ def test_lazily_negated_operands():
         with pytest.raises(_lib.DfsfmError, match="resolve_neg"):
             ops._operands("call", *args)
     assert ops._operands("call", turned.resolve_neg(), (x,), ()) == 0
+
+
+def test_cross_attention_sizes_that_no_launch_holds(built_lib):
+    """A launch holds less than 2^32 threads along an axis.  Sizes at that limit are refused before any launch; the largest below it get as far
+    as the missing workspace."""
+    L = built_lib
+    one = dict(H=1, Hkv=1, nbytes=0)
+    for call in (attention, attention_backward):
+        # tiles of rows, tiles of keys
+        assert call(L, N=64, len=(1 << 25) - 127, S=10, **one) == UNSUPPORTED
+        assert call(L, N=64, len=1, S=(1 << 25) - 127, **one) == UNSUPPORTED and call(L, N=64, len=1, S=(1 << 25) - 128, **one) == WORKSPACE
+    assert attention(L, N=64, len=(1 << 25) - 128, S=10, **one) == WORKSPACE
+    # delta's rows; the forward pass has none
+    assert attention_backward(L, N=1, len=1 << 29, S=10, **one) == UNSUPPORTED and attention(L, N=1, len=1 << 29, S=10, **one) == WORKSPACE
+    assert attention_backward(L, N=1, len=(1 << 29) - 1, S=10, **one) == WORKSPACE
+    assert L.dfsfm_cross_attention_workspace(64, (1 << 25) - 127, 10, 1, 1, 32, 0) == 0
+    assert L.dfsfm_cross_attention_backward_workspace(1, 1 << 29, 10, 1, 1, 32, 0) == 0
