@@ -10,7 +10,7 @@
 // same order of the inner index): the scores never leave the registers.  The query heads that share a key head are rows of one problem: row
 // r is (query r / G, head r % G).
 //
-// Tiles come by LDS-DMA, the next one while this one is worked on.  Keys behind kv_lens are out of the DMA descriptor's range and arrive as
+// Tiles come by LDS-DMA, the next one while this one is worked on, save where waiting for it is faster (Few, attn_dkdv_kernel).  Keys behind kv_lens are out of the DMA descriptor's range and arrive as
 // zeros; rows of LDS whose kv_mask is 0 are cleared; scores of both are set to -inf; a tile without any key is skipped.  Few rows: the keys
 // (or, for dk / dv, the rows) are cut into splits that write 32-bit partial results, joined in a fixed order by a second kernel.  No atomics.
 //
@@ -366,6 +366,22 @@ struct Dma {
 
 __device__ __forceinline__ void dma_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+// Operands that a loop of tiles reads again and again have to be in their registers before it: the compiler knows of their loads but not of
+// the tiles'.  A load that is not settled for it, it waits for in the loop, before the product, until every load is done, the next tile's
+// among them (tests/test_train_edges_cpu.py looks for such waits in the assembly).
+template <typename T, int N>
+__device__ __forceinline__ void settle(Frag<T> (&f)[N]) {
+#pragma unroll
+    for (int s = 0; s < N; ++s) {
+        if constexpr (__is_same(T, X3)) {
+#pragma unroll
+            for (int k = 0; k < 3; ++k) asm volatile("" : "+v"(f[s].p[k]));
+        } else {
+            asm volatile("" : "+v"(f[s]));
+        }
+    }
+}
+
 // Zeros over the rows of a tile whose bit in `keep` is 0, by 256 threads.
 template <typename T, int DP>
 __device__ __forceinline__ void zero_rows(Elem<T>* tile, unsigned long long keep) {
@@ -654,15 +670,22 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_forward_kernel(const
 }
 
 // Up to 32 rows a head, the single-token form: bound by the keys' bytes.  Every wave walks its own tiles of 32 keys through its own ring in
-// LDS, without a barrier, as many tiles ahead as 16 KB hold (two workgroups a CU; 32 KB and one: 72 us against 56 below); the waves' results
-// meet in LDS at the end.  32 single tokens x 8192 keys x 8 x 64 fp16: 95 us, 5.6 TB/s; 16 x 10816 ragged keys: 56 us with the join, 3.6 TB/s
-// (the kernel above, whose four waves share each tile: 117 and 60).
+// LDS, without a barrier; the waves' results meet in LDS at the end.  A workgroup's rings are 64 KB (16 a wave), two workgroups a CU, where
+// that holds two stages or more (16 bits up to 64 channels, fp32 up to 32), and 128 KB, one a CU, for wider rows.  With a mask a turn waits for
+// every tile in flight: its byte is loaded where it is used, and the compiler's wait for it counts no tiles.  32 single tokens x 8192 keys x
+// 8 x 64 fp16: 95 us, 5.6 TB/s; 16 x 10816 ragged keys: 56 us with the join, 3.6 TB/s (the kernel above, whose four waves share each tile: 117
+// and 60), 81 with a mask of two thirds.
 template <typename T, int DP>
 struct Few {
     static constexpr int KT = 32, TILE = KT * DP, STAGE = 2 * TILE * sizeof(T);       // K and V
     static constexpr int WAVES = STAGE > 16384 ? 2 : 4, STAGES = STAGE > 8192 ? 2 : 16384 / STAGE, PITCH = DP + 4;
     static constexpr int RING = WAVES * STAGES * STAGE, JOIN = WAVES * 32 * (PITCH + 4) * 4;
     static constexpr int SMEM = RING > JOIN ? RING : JOIN;
+    // Where two workgroups of two stages share a CU, q is left unsettled: the compiler's wait then takes the next tile in, between the reads of
+    // this one and their products.  32 tokens x 8192 x 8 x 64 fp16 take 98 us so, 104 with the products beside the next tile's fetch, 16 x
+    // 4096 x 8 x 32 fp32 37 and 38.  With more stages, or one workgroup, it is the other way: 32 x 8192 x 8 x 32 bf16 84 and 82, x 128 fp16
+    // 181 and 178, 16 x 8192 x 8 x 64 fp32 132 and 116.
+    static constexpr bool NEXT_TOO = STAGES == 2 && RING == 65536;
 };
 template <typename T, int DP>
 __global__ __launch_bounds__((64 * Few<T, DP>::WAVES)) void attn_forward_few_kernel(const Attn a) {
@@ -696,7 +719,8 @@ __global__ __launch_bounds__((64 * Few<T, DP>::WAVES)) void attn_forward_few_ker
         dv.issue(vb + s0 * a.v.l, end - s0, at + TILE);
     };
     Softmax<T, DP, KT, ROUNDS<T>> sm(a.scale);
-    dma_landed();                           // q is here: from now on the counter counts tiles
+    if constexpr (F::NEXT_TOO) dma_landed();
+    else settle<T>(qf);                     // q is here: from now on the counter counts tiles
 #pragma unroll
     for (int i = 0; i < NS - 1; ++i)
         if (beg + i * KT * NW < end) fetch(beg + i * KT * NW, i);
@@ -1123,6 +1147,12 @@ __global__ __launch_bounds__((64 * KEY_WAVES<T, DP>), (KEY_WAVES<T, DP> / 4)) vo
             dv.issue(static_cast<const Elem<T>*>(a.vt.p) + job.n * a.vt.n + job.hk * a.vt.h + s0 * a.vt.l, len - s0, vs);
         }
         fetch(beg, 0);
+    }
+    // Behind the first fetch, which the loop waits for at once.  2 x 4800 x 4800 x 8 x 64 bf16 forward and gradient 562 -> 557 us, x 128 fp16
+    // 1108 -> 1104.  Unsettled, D = 32 (130 us, 132 settled) and two operands (16 tokens x 10816 x 8 x 64: 176, 178) do a little better.
+    if constexpr (ROUNDS<T> && DP >= 64 && !FINE) {
+        settle<T>(kf);
+        if constexpr (!VLDS) settle<T>(vf);
     }
     const bool mine = __ballot(there) != 0;
     int buf = 0;

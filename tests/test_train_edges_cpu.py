@@ -1,4 +1,7 @@
 """Layer norm, rotary positions and cross attention without a GPU: what their entry points refuse at the edges of what they document."""
+import os
+import re
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -46,3 +49,50 @@ def test_cross_attention_sizes_that_no_launch_holds(built_lib):
     assert attention_backward(L, N=1, len=(1 << 29) - 1, S=10, **one) == WORKSPACE
     assert L.dfsfm_cross_attention_workspace(64, (1 << 25) - 127, 10, 1, 1, 32, 0) == 0
     assert L.dfsfm_cross_attention_backward_workspace(1, 1 << 29, 10, 1, 1, 32, 0) == 0
+
+
+def waits_before_products(listing):
+    """{kernel: number of waits for loads that the compiler, not inline assembly, put before a product in its basic block}, of kernels that
+    fetch tiles by LDS-DMA."""
+    found, name, inline, wait = {}, None, False, False
+    for line in listing:
+        line = line.strip()
+        label = re.match(r"(_Z\w*attn_\w+):", line)
+        if label:
+            name, tiles, count, wait = label.group(1), False, 0, False
+        if name is None:
+            continue
+        if line.startswith(";;#ASMSTART") or line.startswith(";;#ASMEND"):
+            inline = line.startswith(";;#ASMSTART")
+        elif re.match(r"\.LBB\w+:|s_c?branch", line):
+            wait = False
+        elif line.startswith("buffer_load") and line.endswith(" lds"):
+            tiles = True
+        elif line.startswith("s_waitcnt") and "vmcnt" in line:
+            wait = not inline
+        elif line.startswith("v_mfma") and wait:
+            count, wait = count + 1, False
+        elif line.startswith("s_endpgm"):
+            if tiles:
+                found[name] = count
+            name = None
+    return found
+
+
+def test_waits_are_found():
+    code = ["_Z3attn_a:", ";;#ASMSTART", "buffer_load_dwordx4 v1, s[0:3], 0 offen lds", ";;#ASMEND", ".LBB0_1:", "s_waitcnt vmcnt(0) lgkmcnt(1)", "v_mfma_x", "s_endpgm",
+            "_Z3attn_b:", "buffer_load_dwordx4 v1, s[0:3], 0 offen lds", ";;#ASMSTART", "s_waitcnt vmcnt(0)", ";;#ASMEND", "v_mfma_x", "s_waitcnt vmcnt(0)", ".LBB1_2:",
+            "v_mfma_x", "s_endpgm", "_Z3attn_c:", "s_waitcnt vmcnt(0)", "v_mfma_x", "s_endpgm"]
+    assert waits_before_products(code) == {"_Z3attn_a": 1, "_Z3attn_b": 0}
+
+
+def test_products_do_not_wait_for_the_next_tile(built_lib):
+    """In the assembly of the build that is loaded: a tile's products run beside the next tile's fetch in every kernel and instance of cross
+    attention that is not left to wait on purpose (csrc/cross_attention.hip, Few::NEXT_TOO and the settled operands of attn_dkdv_kernel)."""
+    listing = os.path.join(os.path.dirname(_lib.__file__), "csrc", "build", "cross_attention.s")
+    with open(listing) as f:
+        found = waits_before_products(f)
+    waiting = re.compile(r"attn_forward_few_kernelI(DF16[b_]Li64|fLi32)E|attn_dkdv_kernelI(fLi\d+|DF16[b_]Li32)ELb|attn_dkdv_kernelIDF16[b_]Li\d+ELb1")
+    for kernel, least in (("attn_forward_kernel", 12), ("attn_forward_few_kernel", 6), ("attn_dq_kernel", 40), ("attn_dkdv_kernel", 7)):
+        checked = {n: c for n, c in found.items() if kernel in n and not waiting.search(n)}
+        assert len(checked) >= least and not any(checked.values()), (kernel, checked)
