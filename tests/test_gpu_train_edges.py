@@ -6,8 +6,9 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 from detectorfreesfm_amd import _lib, ops
-from test_gpu_cross_attention import TYPES, U, close, rounded
+from test_gpu_cross_attention import TYPES, U, both, check, close, rounded
 from test_gpu_train_norm import rotary_reference
+from test_train_edges_cpu import filled
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -81,6 +82,19 @@ def test_fp16_weights_far_below_the_largest(built_lib, L, S, D, H):
     got, lse = ops.cross_attention(*(x.to(DEV).expand(-1, -1, H, -1) for x in (q, k, v)), scale=1.0)
     close(got, out.expand(1, L, H, D), rounded(out, bound, torch.float16).expand(1, L, H, D), (L, S, D))
     assert float((lse.double().cpu() - torch.log(total)).abs().max()) < (S + 40) * U
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("mask", ["lens", "both"])
+@pytest.mark.parametrize("shape", [(1, 1, 513, 2, 2, 64), (1, 130, 1500, 1, 1, 32), (1, 2000, 40, 1, 1, 64), (3, 1, 1896, 1, 1, 40), (1, 1, 9001, 1, 1, 64),
+                                   (1, 4, 4500, 8, 1, 32), (1, 100, 257, 2, 2, 128), (1, 257, 513, 5, 1, 96), (1, 33, 64, 2, 1, 16), (1, 129, 1500, 1, 1, 128),
+                                   (5, 60, 700, 2, 1, 64), (70, 1, 300, 2, 1, 32)])
+def test_cross_attention_of_sequences_that_all_have_keys(built_lib, shape, mask, t):
+    """Lengths and masks of few sequences, one above all, with keys in each: splits, joins and partial sums of results that are not zero."""
+    q, k, v, do, lens, km, there = filled(*shape, t, mask, sum(shape) + 3)
+    got = both(q, k, v, do, lens, km)
+    assert all(bool((got[n] != 0).flatten(1).any(-1).all()) for n in got)
+    check(got, q, k, v, do, there, shape[-1] ** -0.5, (shape, mask, t))
 
 
 def test_rotary_of_more_tokens_than_one_launch_holds(built_lib):

@@ -10,6 +10,29 @@ from detectorfreesfm_amd import _lib, ops
 from test_train_ops_cpu import UNSUPPORTED, WORKSPACE, attention, attention_backward
 
 
+def filled(N, L, S, H, Hkv, D, t, mask, seed):
+    """Inputs on the CPU of which every sequence has keys; padded places hold NaN, inf and the type's lowest value."""
+    g = torch.Generator().manual_seed(seed)
+    q, do = (torch.randn((N, L, H, D), generator=g) for _ in range(2))
+    k, v = (torch.randn((N, S, Hkv, D), generator=g) for _ in range(2))
+    q, k, v, do = (x.to(t) for x in (1.5 * q, k, v, do))
+    lens = km = None
+    there = torch.ones((N, S), dtype=torch.bool)
+    if mask in ("lens", "both"):
+        lens = torch.tensor([[(2 * S + 2) // 3, S, S + 9, -(-S // 5)][i % 4] for i in range(N)], dtype=torch.int32)
+        there &= torch.arange(S)[None] < lens[:, None]
+    if mask in ("mask", "both"):
+        km = torch.rand((N, S), generator=g) < 0.7
+        if S > 130:
+            km[:, 64:128] = False                                           # a whole tile
+        km[:, 0] = True
+        there &= km
+    assert bool(there.any(-1).all())
+    junk = torch.tensor([float("nan"), float("inf"), torch.finfo(t).min]).to(t)[torch.arange(S) % 3][None, :, None, None]
+    k, v = (torch.where(there[..., None, None], x, junk) for x in (k, v))
+    return q, k, v, do, lens, km, there
+
+
 def test_operands_with_a_tangent():
     """The check behind every entry point, with gradients recorded or not; without a tangent, or outside of a dual level, tensors pass."""
     x = torch.zeros(3)
