@@ -5,10 +5,11 @@ import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
+import attention_norms as an
 from detectorfreesfm_amd import _lib, ops
 from test_gpu_cross_attention import TYPES, U, both, check, close, rounded
 from test_gpu_train_norm import rotary_reference
-from test_train_edges_cpu import filled
+from test_train_edges_cpu import NORM_CASES, filled
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -95,6 +96,21 @@ def test_cross_attention_of_sequences_that_all_have_keys(built_lib, shape, mask,
     got = both(q, k, v, do, lens, km)
     assert all(bool((got[n] != 0).flatten(1).any(-1).all()) for n in got)
     check(got, q, k, v, do, there, shape[-1] ** -0.5, (shape, mask, t))
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape, mask", NORM_CASES)
+def test_cross_attention_rounds_its_results_alone(built_lib, shape, mask, t):
+    """dq of masked or few keys, or of one tile of rows, and every result of up to 32 rows a head: in the 2-norm, where a second rounding of
+    weights or score gradients shows (tests/attention_norms.py, and the test of it without a GPU)."""
+    q, k, v, do, lens, km, there = filled(*shape, t, mask, sum(shape))
+    got = both(q, k, v, do, lens, km)
+    # above 512 keys delta is <dout, out> with the rounded out, which every key of a row shares
+    c = an.terms(q, k, v, do, there, shape[-1] ** -0.5, out=got["out"] if shape[2] > 512 else None)
+    exact, W = an.products(c, c["p"], c["ds"]), an.spreads(c)
+    for n in ("out", "dq", "dk", "dv") if shape[1] * shape[3] // shape[4] <= 32 else ("dq",):
+        off = float((got[n].double().cpu().permute(0, 2, 1, 3) - exact[n]).norm())
+        assert off < an.allowed(exact[n], W[n], t), (n, off, an.allowed(exact[n], W[n], t))
 
 
 def test_rotary_of_more_tokens_than_one_launch_holds(built_lib):

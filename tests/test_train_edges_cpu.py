@@ -6,8 +6,13 @@ import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
+import attention_norms as an
 from detectorfreesfm_amd import _lib, ops
 from test_train_ops_cpu import UNSUPPORTED, WORKSPACE, attention, attention_backward
+
+
+NORM_CASES = [((2, 300, 700, 2, 1, 32), "mask"), ((1, 129, 1500, 1, 1, 128), "both"), ((6, 200, 2048, 2, 2, 64), "lens"), ((2, 100, 3000, 2, 2, 64), "none"),
+              ((3, 4, 512, 8, 8, 64), "none"), ((6, 32, 300, 1, 1, 48), "both"), ((40, 1, 4, 8, 8, 64), "lens")]
 
 
 def filled(N, L, S, H, Hkv, D, t, mask, seed):
@@ -119,3 +124,24 @@ def test_products_do_not_wait_for_the_next_tile(built_lib):
     for kernel, least in (("attn_forward_kernel", 12), ("attn_forward_few_kernel", 6), ("attn_dq_kernel", 40), ("attn_dkdv_kernel", 7)):
         checked = {n: c for n, c in found.items() if kernel in n and not waiting.search(n)}
         assert len(checked) >= least and not any(checked.values()), (kernel, checked)
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape, mask", NORM_CASES)
+def test_norms_see_a_second_rounding(shape, mask, t):
+    """The bound in the 2-norm lets the two-operand form pass and the form that rounds weights and score gradients once fail, for every result
+    that is a sum over keys or rows."""
+    q, k, v, do, _, _, there = filled(*shape, t, mask, sum(shape))
+    c = an.terms(q, k, v, do, there, shape[-1] ** -0.5)
+    exact, W = an.products(c, c["p"], c["ds"]), an.spreads(c)
+    top = c["p"].amax(-1, keepdim=True)
+
+    def operands(form):
+        """out from weights relative to the row's largest, the gradients from ones relative to the row's sum, as the kernels have them."""
+        return {**an.products(c, form(c["p"], t), form(c["ds"], t)), "out": an.products(c, form(c["p"] / top, t), c["ds"])["out"]}
+    two, once = operands(an.two_operands), operands(an.rounded_to)
+    for n, x in exact.items():
+        limit = an.allowed(x, W[n], t)
+        assert float((two[n].to(t).double() - x).norm()) < limit, n
+        if n != "out" or shape[2] > 16:                                     # of a few weights the largest, 1, is exact
+            assert float((once[n].to(t).double() - x).norm()) > limit, n
