@@ -1785,7 +1785,9 @@ def rotary_frequencies(rotated, base=10000.0, axes=1, scaling="none", factor=1.0
     base^(-p / P) a position, and the factor on the turned values.  ``scaling`` stretches them for sequences ``factor`` times as long
     as the ``trained`` length: "linear" divides every frequency; "ntk" enlarges the base so that the slowest pair is divided by ``factor``
     and the fastest stays; "yarn" keeps pairs that turn 32 times or more over the trained length, divides those that turn once or less,
-    blends between, and scales the values by 0.1 ln(factor) + 1."""
+    blends between, and scales the values by 0.1 ln(factor) + 1.  Its blend is linear in the pair's number, which is the logarithm of the
+    turns, and its limits are where the turns are 32 and 1, not the next whole pairs, as some implementations round them (64 channels,
+    factor 8, 4096: up to 16 % apart); nor is it linear in the turns.  A model trained with one of those takes its own ``inv_freq``."""
     if axes not in (1, 2) or rotated <= 0 or rotated % (2 * axes) or base <= 0 or factor < 1 or scaling not in ("none", "linear", "ntk", "yarn"):
         raise _lib.DfsfmError("rotary_frequencies: rotated channels are 2 * axes * pairs, axes 1 or 2, factor >= 1, scaling one of none, "
                               "linear, ntk, yarn")

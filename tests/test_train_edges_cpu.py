@@ -1,4 +1,5 @@
 """Layer norm, rotary positions and cross attention without a GPU: what their entry points refuse at the edges of what they document."""
+import math
 import os
 import re
 
@@ -145,3 +146,19 @@ def test_norms_see_a_second_rounding(shape, mask, t):
         assert float((two[n].to(t).double() - x).norm()) < limit, n
         if n != "out" or shape[2] > 16:                                     # of a few weights the largest, 1, is exact
             assert float((once[n].to(t).double() - x).norm()) > limit, n
+
+
+@pytest.mark.parametrize("rotated, axes, factor, trained", [(64, 1, 8.0, 4096), (128, 1, 2.0, 2048), (96, 2, 16.0, 8192)])
+def test_rotary_frequencies_yarn_between_its_limits(rotated, axes, factor, trained):
+    """The blend runs linearly in the pair's number from the (fractional) pair that turns 32 times over the trained length to the one that turns
+    once: base^(-p / P) trained / 2 pi = 32 and 1 at p = P log(trained / (2 pi turns)) / log(base)."""
+    P, base = rotated // (2 * axes), 10000.0
+    first, last = (P * math.log(trained / (2 * math.pi * turns)) / math.log(base) for turns in (32.0, 1.0))
+    inv, _ = ops.rotary_frequencies(rotated, base=base, axes=axes, scaling="yarn", factor=factor, trained=trained, device="cpu")
+    between = 0
+    for p in range(P):
+        divided = min(1.0, max(0.0, (p - first) / (last - first)))          # share of the divided frequency
+        between += 0.0 < divided < 1.0
+        want = base ** (-p / P) * ((1.0 - divided) + divided / factor)
+        assert abs(float(inv[p]) - want) < 1e-13 * want, p
+    assert between >= 5
