@@ -1654,6 +1654,7 @@ def maxpool3x3s2_nhwc(x):
 # beside it.  Their smallest calls are bound by this file, not by the GPU: the checks below are written for few Python calls.
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice      # a tensor on a device says that the runtime is up: no check for that a call
 
 
 def _on_first_device(fn):
@@ -1666,7 +1667,7 @@ def _on_first_device(fn):
         x = args[0] if args else kw.get(first)
         if not isinstance(x, torch.Tensor) or not x.is_cuda:
             raise _lib.DfsfmError(f"{fn.__name__}: HIP ops need device tensors (there is no CPU path)")
-        if x.get_device() == torch.cuda.current_device():
+        if x.get_device() == _current_device():
             return fn(*args, **kw)
         with torch.cuda.device(x.get_device()):
             return fn(*args, **kw)
@@ -1675,10 +1676,10 @@ def _on_first_device(fn):
 
 def _operands(what, x, same, others):
     """The type code of x; every tensor of ``same`` has its type, and those of ``others`` too are on its device (None: absent)."""
-    code, dev = _DTYPES.get(x.dtype), x.get_device()
+    dt, dev, graph = x.dtype, x.get_device(), torch.is_grad_enabled()
+    code = _DTYPES.get(dt)
     if code is None:
-        raise _lib.DfsfmError(f"{what}: need fp32, bf16 or fp16 tensors, got {x.dtype}")
-    graph = torch.is_grad_enabled()
+        raise _lib.DfsfmError(f"{what}: need fp32, bf16 or fp16 tensors, got {dt}")
     if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (x, *same, *others)):
         raise _lib.DfsfmError(f"{what}: an operand carries a tangent, which no operator here moves on: call it on the primal tensors")
     for t in (x, *same, *others):
@@ -1692,8 +1693,8 @@ def _operands(what, x, same, others):
             raise _lib.DfsfmError(f"{what}: records no autograd graph: call it on detached tensors (or under torch.no_grad()) and its "
                                   "gradient with the backward function beside it")
     for t in same:
-        if t is not None and t.dtype != x.dtype:
-            raise _lib.DfsfmError(f"{what}: need tensors of one type, got {x.dtype} and {t.dtype}")
+        if t is not None and t.dtype is not dt:
+            raise _lib.DfsfmError(f"{what}: need tensors of one type, got {dt} and {t.dtype}")
     return code
 
 
