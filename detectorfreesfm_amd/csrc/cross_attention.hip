@@ -10,14 +10,17 @@
 // same order of the inner index): the scores never leave the registers.  The query heads that share a key head are rows of one problem: row
 // r is (query r / G, head r % G).
 //
-// Tiles come by LDS-DMA, the next one while this one is worked on, save where waiting for it is faster (Few, attn_dkdv_kernel).  Keys behind kv_lens are out of the DMA descriptor's range and arrive as
-// zeros; rows of LDS whose kv_mask is 0 are cleared; scores of both are set to -inf; a tile without any key is skipped.  Few rows: the keys
-// (or, for dk / dv, the rows) are cut into splits that write 32-bit partial results, joined in a fixed order by a second kernel.  No atomics.
+// Tiles come by LDS-DMA, the next one while this one is worked on, save where waiting for it is faster (Few, attn_dkdv_kernel).  Keys behind
+// kv_lens are out of the DMA descriptor's range and arrive as zeros; rows of LDS whose kv_mask is 0 are cleared; scores of both are set to
+// -inf; a tile without any key is skipped.  Few rows: the keys (or, for dk / dv, the rows) are cut into splits that write 32-bit partial
+// results, joined in a fixed order by a second kernel.  No atomics.
 //
 // What bounds the large cases is the exponentials beside the products: a wave's VALU instructions run at half rate while the other wave of its
-// SIMD streams MFMAs.  4 x 4800 x 6400 keys (ragged) x 16 / 4 heads x 128 bf16: forward 0.73, dq 0.89, dk / dv 1.20 ms, in products 0.85,
-// 1.03 and 1.03 PFLOP/s, where a plain 8192^3 product of the library runs at 1.17; 2 x 4800 x 10816 x 8 x 32 fp32 forward 0.57 ms = 140
-// TFLOP/s (library: 154).
+// SIMD streams MFMAs.  4 x 4800 x 6400 keys (ragged) x 16 / 4 heads x 128 bf16: forward 0.69 - 0.74, dq 0.85 - 0.89, dk / dv 1.10 - 1.19 ms by
+// the card, in products 0.83 - 0.89, 1.04 - 1.09 and 1.04 - 1.12 PFLOP/s, where a plain 8192^3 product of the library runs at 1.17; the
+// matrix pipes are busy 41, 55 and 52 % of the time.  fp32, 2 x 4800 x 4800 x 8 heads: forward at D = 32 295 us = 160 TFLOP/s, 64 495 = 190,
+// 128 1100 = 172 (library: 154), with the gradient 1.18, 2.13 and 4.67 ms = 140, 154 and 141; D = 40, 80 and 96 pay for 64, 128 and 128
+// (0.45, 1.03 and 1.04 ms forward): blocks of channels that are not there are multiplied, since the chunk order in LDS takes powers of two.
 #include "elem.h"
 
 namespace {
@@ -150,7 +153,8 @@ __device__ __forceinline__ Frag<T> load8(const Mem<T>* p) {
 // by LDS-DMA, 1 KB of consecutive LDS an instruction); their 16-byte chunks are permuted by the row number: chunk c of row r lies at c ^
 // order(r), where order() differs by at least four chunks between neighbouring rows that share banks (the transposed read) and takes every
 // value over 16 rows (the other).  A lane's row is the same modulo 16 in every read, so the permutation is one exclusive or with a
-// constant.  Padded rows (272 or 288 bytes) cost the dk / dv kernel 35 % of its LDS cycles in conflicts; this order has none.
+// constant.  Padded rows (272 or 288 bytes) cost the dk / dv kernel 35 % of its LDS cycles in conflicts; this order has none, by the counter in
+// every kernel of this file.
 template <typename T, int DP>
 struct LdsPlane {
     static constexpr bool HALF = sizeof(T) == 2;
@@ -303,6 +307,8 @@ struct Job {
     __device__ __forceinline__ explicit Job(const Attn& a) : Job(a, a.tiles, a.splits) {}
     // The same for tiles of `rows` keys, the tiles with keys of every sequence first: workgroups go to XCDs by their number, so tiles that
     // have nothing to do must not lie between the others (4 x 6400 ragged keys: XCDs with four rounds of work beside ones with three).
+    // Every workgroup walks the lengths, which more sequences do not repay: 256 single tokens x 2048 x 8 x 64 take 131 us as they come, 210
+    // sorted, 128 x 512 x 512 forward and gradient 384 and 422; 64 x 512 x 512 206 and 212, 4 x 4800 x 6400 (see above) gains.
     __device__ __forceinline__ Job(const Attn& a, int tiles, int splits, int rows) : Job(a, tiles, splits) {
         if (!a.lens || a.N > 64) return;
         const int hkv = a.H / a.G, per = hkv * splits;
@@ -325,8 +331,8 @@ struct Job {
 __device__ __forceinline__ int valid_len(const Attn& a, int n) { return a.lens ? min(max(a.lens[n], 0), a.S) : a.S; }
 
 // A tile of NROWS rows x DP channels on its way from memory into LDS, by LDS-DMA: no register holds it and no vector instruction moves it.
-// Every one of THREADS threads (the workgroup, or a wave for itself) fetches 16 bytes an instruction; the chunk order of Lds is applied to the source address.  Rows behind the last and channels
-// behind D lie outside the buffer descriptor and arrive as zeros.
+// Every one of THREADS threads (the workgroup, or a wave for itself) fetches 16 bytes an instruction; the chunk order of Lds is applied to the
+// source address.  Rows behind the last and channels behind D lie outside the buffer descriptor and arrive as zeros.
 template <typename T, int DP, int NROWS, int THREADS>
 struct Dma {
     typedef LdsPlane<Elem<T>, DP> L;
@@ -673,8 +679,8 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_forward_kernel(const
 // LDS, without a barrier; the waves' results meet in LDS at the end.  A workgroup's rings are 64 KB (16 a wave), two workgroups a CU, where
 // that holds two stages or more (16 bits up to 64 channels, fp32 up to 32), and 128 KB, one a CU, for wider rows.  With a mask a turn waits for
 // every tile in flight: its byte is loaded where it is used, and the compiler's wait for it counts no tiles.  32 single tokens x 8192 keys x
-// 8 x 64 fp16: 95 us, 5.6 TB/s; 16 x 10816 ragged keys: 56 us with the join, 3.6 TB/s (the kernel above, whose four waves share each tile: 117
-// and 60), 81 with a mask of two thirds.
+// 8 x 64 fp16: 98 us, 5.5 TB/s; 16 x 10816 ragged keys: 52 - 59 us with the join, 3.4 - 3.9 TB/s (the kernel above, whose four waves share
+// each tile: 117 and 60), 81 with a mask of two thirds.
 template <typename T, int DP>
 struct Few {
     static constexpr int KT = 32, TILE = KT * DP, STAGE = 2 * TILE * sizeof(T);       // K and V
@@ -1078,7 +1084,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(const Attn
 //
 // NW is 4, two workgroups a CU, where a wave's K, V, dk and dv leave room for two waves a SIMD.  At D = 128 in 16 bits they are 192 registers
 // before the first score; there NW is 8, one workgroup a CU, and V stays in LDS (64 KB for 256 keys), read again for every tile.
-// 4 x 4800 x 6400 (ragged) x 16 heads bf16 takes 1.21 - 1.31 ms; with V in registers, four waves and one wave a SIMD 2.3; with the two halves
+// 4 x 4800 x 6400 (ragged) x 16 heads bf16 takes 1.10 - 1.19 ms; with V in registers, four waves and one wave a SIMD 2.3; with the two halves
 // of the work on two waves that pass p through LDS 1.7; as two launches, one product made twice, 1.8.
 template <typename T, int DP>
 constexpr int KEY_WAVES = DP == 128 && sizeof(Mem<T>) == 2 ? 8 : 4;
@@ -1252,9 +1258,10 @@ bool rows_ok(const void* p, int64_t n, int64_t l, int64_t h, int D, int dtype) {
     return !((uintptr_t)p & 15) && n % e == 0 && l % e == 0 && h % e == 0 && l >= D && l < (1ll << 23);
 }
 
-// Splits of the long axis (`length` rows of it, `least` a split).  `slots` workgroups run at a time (512: two a CU); as long as they number
-// less than eight such rounds the last one's idle places count, and the smallest number of splits that fills 85 % of the places is taken: 608
-// workgroups of the forward pass 2 x 4800 x 10816 x 8 x 32 fp32 take 1.21 ms, three splits of each 0.98 with the join.
+// Splits of the long axis (`length` rows of it, `least` a split).  `slots` workgroups run at a time (512: two a CU; of instances that leave
+// room for one, two rounds); as long as they number less than eight such rounds the last one's idle places count, and the smallest number of
+// splits that fills 85 % of the places is taken: 608 workgroups of the forward pass 2 x 4800 x 10816 x 8 x 32 fp32 take 637 us, three splits of
+// each 530 - 570 with planes and join.
 // A join is 5 us, what 256 keys of 16 bits take a wave; of fp32's products (32 keys of 128 channels: 3 us in planes, 5 on the 32-bit
 // instruction) 64 keys are worth one: 33 x 1387 x 4 x 80 forward and gradient 140 -> 81 us, one row of 4 x 3271 keys 120 -> 76.
 int choose_splits(int64_t groups, int64_t length, int slots, int least) {
@@ -1287,8 +1294,9 @@ struct Plan {
         tq = (int)((R + 127) / 128);
         tk = (S + wave_keys - 1) / wave_keys;
         few = R <= 32;
-        // Few rows read their keys once, from memory: about a workgroup a CU does without the join (256 heads x 8192 x 64 fp16: 95 us against
-        // 110 in two splits), below that two a CU (128 heads x 10816 ragged keys: 56 us in four splits, 66 in two, 57 in eight).
+        // Few rows read their keys once, from memory: about a workgroup a CU does without the join (256 heads x 8192 x 64 fp16: 98 us against
+        // 110 in two splits, x 128 bf16 178 and 186), below that two a CU (128 heads x 10816 ragged keys x 64: 53 us in four splits, 68 in two,
+        // 54 in eight; x 128 bf16 95, 91 and 87, x 32 45, 43 and 35).
         fwd = few && heads >= 200 ? 1 : choose_splits((int64_t)heads * tq, S, tq == 1 && !few ? 2048 : 512, least);
         dq = S <= (dtype == DFSFM_F32 ? 128 : EXACT_KEYS) ? 1 : choose_splits((int64_t)heads * tq, S, tq == 1 ? 2048 : 512, least);
         dkdv = choose_splits((int64_t)heads * tk, R, wave_keys == 256 ? 256 : 512, least);
